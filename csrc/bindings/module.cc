@@ -1,5 +1,6 @@
 // pybind11 module `seldon_core_amd._C`: the native engine, front ends, GPU
 // units and raw kernel launchers.
+#include <array>
 #include <pybind11/numpy.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
@@ -21,6 +22,7 @@
 #include "../gpu/models.h"
 #include "../gpu/router.h"
 #include "../kernels/kernels.h"
+#include "../kernels/token_step.h"
 #include "../parallel/fabric.h"
 #include "../parallel/mesh.h"
 #include "../server/grpc_server.h"
@@ -1137,6 +1139,62 @@ PYBIND11_MODULE(_C, m) {
   k.def("ts_route", [](uintptr_t alpha, uintptr_t beta, int nb, uint64_t seed, uint64_t offset, int n, uintptr_t out,
                        uintptr_t s) {
     kern::ts_route(P<const float>(alpha), P<const float>(beta), nb, seed, offset, n, P<double>(out), as_stream(s));
+  });
+
+  // token serving: strides in elements, as torch has them
+  k.def("qk_norm_rope", [](uintptr_t q, uintptr_t k_, uintptr_t oq, uintptr_t ok, uintptr_t qw, uintptr_t kw, bool w_f32,
+                           const std::array<int64_t, 8>& st, int64_t tokens, int hq, int hk, int dim, int type,
+                           uintptr_t pos, int pos64, uintptr_t inv, int inv64, int n_freq, bool interleaved, float eps,
+                           uintptr_t s) {
+    kern::QkNormRopeArgs a;
+    a.x[0] = P<const void>(q), a.x[1] = P<const void>(k_);
+    a.out[0] = P<void>(oq), a.out[1] = P<void>(ok);
+    a.weight[0] = P<const void>(qw), a.weight[1] = P<const void>(kw);
+    a.heads[0] = hq, a.heads[1] = hk;
+    for (int i = 0; i < 2; ++i) {
+      a.x_token[i] = st[size_t(2 * i)], a.x_head[i] = st[size_t(2 * i + 1)];
+      a.out_token[i] = st[size_t(4 + 2 * i)], a.out_head[i] = st[size_t(5 + 2 * i)];
+    }
+    a.tokens = tokens, a.dim = dim, a.type = type, a.weight_f32 = w_f32;
+    a.positions = P<const void>(pos), a.positions64 = pos64;
+    a.inv_freq = P<const void>(inv), a.inv_freq64 = inv64, a.n_freq = n_freq;
+    a.interleaved = interleaved, a.eps = eps;
+    kern::qk_norm_rope(a, as_stream(s));
+  });
+
+  // x: k, v; cache: k, v, k scales, v scales; cst: strides of the four caches' first three dimensions
+  const auto kv_args = [](const std::array<uintptr_t, 2>& x, const std::array<int64_t, 4>& xst, int type,
+                          const std::array<uintptr_t, 4>& cache, const std::array<int64_t, 12>& cst, int cache_type,
+                          int64_t pages, int64_t page_size, uintptr_t slots, int slots64, int64_t rows, int heads, int dim) {
+    kern::KvCacheArgs a;
+    for (size_t i = 0; i < 2; ++i) {
+      a.x[i] = P<void>(x[i]);
+      a.x_row[i] = xst[2 * i], a.x_head[i] = xst[2 * i + 1];
+      a.cache[i] = P<void>(cache[i]);
+      a.c_page[i] = cst[3 * i], a.c_slot[i] = cst[3 * i + 1], a.c_head[i] = cst[3 * i + 2];
+      a.scale[i] = P<float>(cache[2 + i]);
+      a.s_page[i] = cst[6 + 3 * i], a.s_slot[i] = cst[7 + 3 * i], a.s_head[i] = cst[8 + 3 * i];
+    }
+    if (page_size < 1 || page_size > 0x7fffffff) throw std::invalid_argument("kv_cache: page size");
+    a.type = type, a.cache_type = cache_type;
+    a.slots = P<const void>(slots), a.slots64 = slots64;
+    a.page = kern::FastDiv(uint32_t(page_size)), a.slots_total = pages * page_size;
+    a.rows = rows, a.heads = heads, a.dim = dim;
+    return a;
+  };
+  k.def("kv_cache_write", [kv_args](const std::array<uintptr_t, 2>& x, const std::array<int64_t, 4>& xst, int type,
+                                    const std::array<uintptr_t, 4>& cache, const std::array<int64_t, 12>& cst,
+                                    int cache_type, int64_t pages, int64_t page_size, uintptr_t slots, int slots64,
+                                    int64_t rows, int heads, int dim, uintptr_t s) {
+    kern::kv_cache_write(kv_args(x, xst, type, cache, cst, cache_type, pages, page_size, slots, slots64, rows, heads, dim),
+                         as_stream(s));
+  });
+  k.def("kv_cache_read", [kv_args](const std::array<uintptr_t, 2>& x, const std::array<int64_t, 4>& xst, int type,
+                                   const std::array<uintptr_t, 4>& cache, const std::array<int64_t, 12>& cst,
+                                   int cache_type, int64_t pages, int64_t page_size, uintptr_t slots, int slots64,
+                                   int64_t rows, int heads, int dim, uintptr_t s) {
+    kern::kv_cache_read(kv_args(x, xst, type, cache, cst, cache_type, pages, page_size, slots, slots64, rows, heads, dim),
+                        as_stream(s));
   });
 
   // ------------------------------------------------------------- remote nodes

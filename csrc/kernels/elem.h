@@ -1,0 +1,116 @@
+// Element types of the token-serving kernels (rope, kv_cache, paged_attention,
+// lora): loads and stores of short runs through fp32, row addressing in a
+// paged cache, and lane-group reductions.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "token_step.h"
+
+namespace sca::kern {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+struct e4m3 {
+  uint8_t bits;
+};
+
+template <class T> constexpr bool kQuantised = sizeof(T) == 1;
+
+// V consecutive elements as fp32.  The pointer is aligned to
+// min(16, V * sizeof(T)) bytes: one vector load for each 16 bytes.
+template <int V, class T> __device__ __forceinline__ void load_run(const T* p, float* f) {
+  if constexpr (std::is_same_v<T, e4m3>) {
+    if constexpr (V % 4 == 0) {
+      using U = uint32_t __attribute__((ext_vector_type(V / 4)));
+      const U u = *reinterpret_cast<const U*>(p);
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) {
+        uint32_t w;
+        if constexpr (V == 4) w = *reinterpret_cast<const uint32_t*>(&u);
+        else w = u[i];
+        f[4 * i + 0] = __builtin_amdgcn_cvt_f32_fp8(int(w), 0);
+        f[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(int(w), 1);
+        f[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(int(w), 2);
+        f[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(int(w), 3);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = __builtin_amdgcn_cvt_f32_fp8(int(p[i].bits), 0);
+    }
+  } else {
+    constexpr int N = V * int(sizeof(T)) > 16 ? 16 / int(sizeof(T)) : V;  // elements of one load
+    using U = T __attribute__((ext_vector_type(N)));
+#pragma unroll
+    for (int j = 0; j < V; j += N) {
+      if constexpr (N == 1) {
+        f[j] = float(p[j]);
+      } else {
+        const U u = *reinterpret_cast<const U*>(p + j);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[j + i] = float(u[i]);
+      }
+    }
+  }
+}
+
+// The reverse, rounded to nearest even.  e4m3 and int8 take values that are in
+// range already; NaN gives e4m3's NaN and int8's 0.
+template <int V, class T> __device__ __forceinline__ void store_run(T* p, const float* f) {
+  if constexpr (std::is_same_v<T, e4m3>) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < V; i += 8) {
+        uint32_t w[2];
+#pragma unroll
+        for (int j = 0; j < 2 && i + 4 * j < V; ++j) {
+          int u = __builtin_amdgcn_cvt_pk_fp8_f32(f[i + 4 * j], f[i + 4 * j + 1], 0, false);
+          u = __builtin_amdgcn_cvt_pk_fp8_f32(f[i + 4 * j + 2], f[i + 4 * j + 3], u, true);
+          w[j] = uint32_t(u);
+        }
+        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+        else *reinterpret_cast<uint2*>(p + i) = make_uint2(w[0], w[1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[i].bits = uint8_t(__builtin_amdgcn_cvt_pk_fp8_f32(f[i], 0.f, 0, false) & 0xff);
+    }
+  } else {
+    constexpr int N = V * int(sizeof(T)) > 16 ? 16 / int(sizeof(T)) : V;
+    using U = T __attribute__((ext_vector_type(N)));
+#pragma unroll
+    for (int j = 0; j < V; j += N) {
+      if constexpr (N == 1) {
+        p[j] = T(f[j]);
+      } else {
+        U u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = T(f[j + i]);
+        *reinterpret_cast<U*>(p + j) = u;
+      }
+    }
+  }
+}
+
+// Sum / largest over the `width` (a power of two) neighbouring lanes of a group.
+__device__ __forceinline__ float group_sum(float v, int width) {
+  for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// NaN stays NaN.
+__device__ __forceinline__ float group_max(float v, int width) {
+  for (int o = width >> 1; o > 0; o >>= 1) {
+    const float w = __shfl_xor(v, o);
+    v = (w > v || w != w) ? w : v;
+  }
+  return v;
+}
+
+__device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i) {
+  return is64 ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
+}
+
+}  // namespace sca::kern

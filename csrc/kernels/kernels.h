@@ -432,33 +432,4 @@ struct LstmvProgram {
 void lstm_valu_mse(const double* X, int rows, const LstmvProgram& prog, const float* params, double* out,
                    hipStream_t stream);
 
-// ---------------------------------------------------------------- token serving
-// Operators of one step of a served token model (rope.hip, kv_cache.hip,
-// paged_attention.hip, lora.hip).  Strides count elements; the last dimension
-// of every tensor is contiguous.  Launchers throw std::invalid_argument for
-// what they do not take and std::runtime_error for a launch that fails.
-enum ElemType : int { kF32 = 0, kF16 = 1, kBF16 = 2, kE4M3 = 3, kI8 = 4 };
-
-// RMS norm of each head of q and k, then rotation of its first 2 * n_freq
-// dimensions by pos * inv_freq, in one launch for both.
-struct QkNormRopeArgs {
-  const void* x[2] = {};        // q, k: [tokens, heads[i], dim]
-  void* out[2] = {};            // may be x
-  const void* weight[2] = {};   // [dim] or null (no learned weight)
-  int heads[2] = {};
-  int64_t x_token[2] = {}, x_head[2] = {}, out_token[2] = {}, out_head[2] = {};
-  int64_t tokens = 0;
-  int dim = 0;                  // even, <= 512
-  int type = kBF16;             // of x and out: kF32, kF16 or kBF16
-  int weight_f32 = 0;           // weights are fp32, not `type`
-  const void* positions = nullptr;  // [tokens] int32 or int64
-  int positions64 = 0;
-  const void* inv_freq = nullptr;   // [n_freq] fp32 or fp64, radians per position
-  int inv_freq64 = 0;
-  int n_freq = 0;               // rotated pairs, <= dim / 2
-  int interleaved = 0;          // pairs (2i, 2i + 1), else (i, i + n_freq)
-  float eps = 1e-6f;
-};
-void qk_norm_rope(const QkNormRopeArgs& a, hipStream_t stream);
-
 }  // namespace sca::kern

@@ -1,0 +1,26 @@
+// A kernel launch whose own error is reported (not one that an earlier call left).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stdexcept>
+#include <string>
+#include <tuple>
+#include <utility>
+
+namespace sca::kern {
+
+template <class... P, class... A>
+void launch_kernel(void (*fn)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t s, A&&... args) {
+  static_assert(sizeof...(P) == sizeof...(A), "one argument for each parameter");
+  std::tuple<std::decay_t<P>...> held(std::forward<A>(args)...);
+  std::apply(
+      [&](auto&... x) {
+        void* ptrs[] = {const_cast<void*>(static_cast<const void*>(&x))...};
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(fn), grid, block, ptrs, lds, s);
+        if (e != hipSuccess) throw std::runtime_error(std::string("kernel launch failed: ") + hipGetErrorString(e));
+      },
+      held);
+}
+
+}  // namespace sca::kern

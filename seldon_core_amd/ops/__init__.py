@@ -6,13 +6,15 @@ orders with surrounding torch work and can be captured in a hipGraph).  There
 is no silent fallback: calling an op on CPU tensors or without the native
 extension raises.  CPU references for the tests live next to each op.
 
-Kernel sources: csrc/kernels/{linear,combine,image,tree,bandit}.hip.
+Kernel sources: csrc/kernels/{linear,combine,image,tree,bandit}.hip; the
+operators of served token models are in :mod:`.token_step`.
 """
 from __future__ import annotations
 
 from typing import List, Sequence
 
 from .._native import native
+from .token_step import KVCache, kv_cache, kv_cache_read, kv_cache_write, qk_norm_rope  # noqa: F401
 
 
 def _k():
