@@ -1197,6 +1197,53 @@ PYBIND11_MODULE(_C, m) {
                         as_stream(s));
   });
 
+  // q, the cache and its strides as kv_cache_write has them; ws: fp32 workspace of ws_floats
+  k.def("paged_attention", [](uintptr_t q, int64_t q_batch, int64_t q_head, int type, const std::array<uintptr_t, 4>& cache,
+                              const std::array<int64_t, 12>& cst, int cache_type, int64_t pages, int64_t page_size,
+                              uintptr_t table, int64_t table_row, int64_t table_width, uintptr_t lengths, int batch,
+                              int kv_heads, int group, int dim, int window, float scale, uintptr_t out, uintptr_t lse,
+                              uintptr_t ws, int64_t ws_floats, uintptr_t s) {
+    if (page_size < 1 || page_size > 0x7fffffff || pages > 0x7fffffff || table_width > (int64_t(1) << 30))
+      throw std::invalid_argument("paged_attention: sizes");
+    kern::PagedAttentionArgs a;
+    a.q = P<const void>(q), a.q_batch = q_batch, a.q_head = q_head, a.type = type;
+    a.q_vector = q % 16 == 0 && q_batch % 8 == 0 && q_head % 8 == 0;
+    for (size_t i = 0; i < 2; ++i) {
+      a.cache[i] = P<const void>(cache[i]);
+      a.c_page[i] = cst[3 * i], a.c_slot[i] = cst[3 * i + 1], a.c_head[i] = cst[3 * i + 2];
+      a.cache_scale[i] = P<const float>(cache[2 + i]);
+      a.s_page[i] = cst[6 + 3 * i], a.s_slot[i] = cst[7 + 3 * i], a.s_head[i] = cst[8 + 3 * i];
+    }
+    a.cache_type = cache_type;
+    a.table = P<const int32_t>(table), a.table_row = table_row, a.lengths = P<const int32_t>(lengths);
+    a.pages = int(pages), a.page = kern::FastDiv(uint32_t(page_size));
+    a.max_tokens = int(std::min(table_width * page_size, int64_t(0x7fffffff)));
+    a.batch = batch, a.kv_heads = kv_heads, a.group = group, a.dim = dim, a.window = window, a.scale = scale;
+    a.out = P<void>(out), a.lse = P<float>(lse);
+    if (kern::paged_attention_plan(a) > ws_floats) throw std::invalid_argument("paged_attention: workspace too small");
+    a.partial_ml = P<float>(ws);
+    a.partial_o = P<float>(ws) + 4 * int64_t(a.grid) * a.partial_rows;
+    kern::paged_attention(a, as_stream(s));
+  });
+  k.def("paged_attention_workspace", &kern::paged_attention_workspace, "fp32 numbers of workspace");
+
+  k.def("lora_add", [](uintptr_t y, int64_t y_row, uintptr_t x, int64_t x_row, uintptr_t out, int64_t out_row, uintptr_t A,
+                       uintptr_t B, uintptr_t ids, int ids64, uintptr_t scales, int64_t rows, int64_t inner, int64_t outer,
+                       int64_t rank, int64_t adapters, int type, uintptr_t ws, int64_t ws_floats, uintptr_t s) {
+    if (std::max({inner, outer, rank, adapters}) > 0x7fffffff) throw std::invalid_argument("lora_add: sizes");
+    kern::LoraArgs a;
+    a.x = P<const void>(x), a.y = P<const void>(y), a.out = P<void>(out);
+    a.x_row = x_row, a.y_row = y_row, a.out_row = out_row;
+    a.A = P<const void>(A), a.B = P<const void>(B);
+    a.ids = P<const void>(ids), a.ids64 = ids64, a.scales = P<const float>(scales);
+    a.rows = rows, a.inner = int(inner), a.outer = int(outer), a.rank = int(rank), a.adapters = int(adapters), a.type = type;
+    if (rows > 0 && kern::lora_workspace(rows, a.inner, a.rank) > ws_floats)
+      throw std::invalid_argument("lora_add: workspace too small");
+    a.h = P<float>(ws);
+    kern::lora_add(a, as_stream(s));
+  });
+  k.def("lora_workspace", &kern::lora_workspace, "fp32 numbers of workspace");
+
   // ------------------------------------------------------------- remote nodes
   py::class_<RemoteUnit, Unit, std::shared_ptr<RemoteUnit>>(m, "RemoteUnit")
       .def(py::init([](const std::string& host, int port, bool grpc, const std::string& node_type,

@@ -17,7 +17,10 @@ void launch_kernel(void (*fn)(P...), dim3 grid, dim3 block, size_t lds, hipStrea
   std::apply(
       [&](auto&... x) {
         void* ptrs[] = {const_cast<void*>(static_cast<const void*>(&x))...};
-        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(fn), grid, block, ptrs, lds, s);
+        hipError_t e = hipSuccess;
+        if (lds > 64 * 1024)  // beyond the default limit of a launch
+          e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+        if (e == hipSuccess) e = hipLaunchKernel(reinterpret_cast<const void*>(fn), grid, block, ptrs, lds, s);
         if (e != hipSuccess) throw std::runtime_error(std::string("kernel launch failed: ") + hipGetErrorString(e));
       },
       held);

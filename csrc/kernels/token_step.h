@@ -74,4 +74,60 @@ struct KvCacheArgs {
 void kv_cache_write(const KvCacheArgs& a, hipStream_t stream);
 void kv_cache_read(const KvCacheArgs& a, hipStream_t stream);
 
+// Attention of one new token for each request over a paged cache.  A token whose
+// page is outside the cache is left out; a request that sees no token gets zeros
+// and a logsumexp of -infinity.
+struct PagedAttentionArgs {
+  const void* q = nullptr;      // [batch, kv_heads * group, dim]
+  int64_t q_batch = 0, q_head = 0;
+  int q_vector = 0;             // its rows start at multiples of 16 bytes
+  int type = kBF16;             // of q and out: kF16 or kBF16
+  const void* cache[2] = {};    // k, v: [pages, page size, kv_heads, dim], of `type` or 8 bits
+  int64_t c_page[2] = {}, c_slot[2] = {}, c_head[2] = {};
+  int cache_type = kBF16;
+  const float* cache_scale[2] = {};  // [pages, page size, kv_heads]
+  int64_t s_page[2] = {}, s_slot[2] = {}, s_head[2] = {};
+  const int32_t* table = nullptr;    // [batch, max_tokens / page size] pages
+  int64_t table_row = 0;
+  const int32_t* lengths = nullptr;  // [batch] tokens
+  int pages = 0;
+  FastDiv page;
+  int max_tokens = 0;           // what a row of the table holds: longer lengths count as this
+  int batch = 0, kv_heads = 0, group = 0, dim = 0;
+  int window = 0;               // the last tokens that a request sees; 0: all
+  float scale = 1.f;
+  void* out = nullptr;          // [batch, kv_heads * group, dim], contiguous
+  float* lse = nullptr;         // [batch, kv_heads * group] natural logsumexp of the scores, or null
+  // filled in by paged_attention_plan()
+  int q_heads = 0, row_blocks = 0, partial_rows = 0, grid = 0;
+  float* partial_o = nullptr;   // [2 grid, partial_rows, padded dim]
+  float* partial_ml = nullptr;  // [2 grid, partial_rows, 2]
+};
+// Checks the arguments, chooses the grid and returns the workspace in floats:
+// partial_ml lies at its start, partial_o behind its 4 * grid * partial_rows floats.
+int64_t paged_attention_plan(PagedAttentionArgs& a);
+void paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
+int64_t paged_attention_workspace(int batch, int kv_heads, int group, int dim, int64_t max_tokens, int window);
+
+// out = y + scale[a] * (x A[a]^T) B[a]^T for each row's adapter a.
+struct LoraArgs {
+  const void* x = nullptr;      // [rows, inner]
+  const void* y = nullptr;      // [rows, outer]
+  void* out = nullptr;          // [rows, outer], may be y
+  int64_t x_row = 0, y_row = 0, out_row = 0;
+  const void* A = nullptr;      // [adapters, rank, inner], contiguous
+  const void* B = nullptr;      // [adapters, outer, rank], contiguous
+  const void* ids = nullptr;    // [rows] int32 or int64; one that is no adapter leaves its row as y has it
+  int ids64 = 0;
+  const float* scales = nullptr;  // [adapters] or null
+  int64_t rows = 0;
+  int inner = 0, outer = 0, rank = 0, adapters = 0;
+  int type = kBF16;             // of all but ids and scales: kF32, kF16 or kBF16
+  float* h = nullptr;           // workspace of lora_workspace() floats
+  // filled in by lora_add()
+  int splits = 1, col_tiles = 1, vector = 0;
+};
+int64_t lora_workspace(int64_t rows, int inner, int rank);
+void lora_add(LoraArgs a, hipStream_t stream);
+
 }  // namespace sca::kern

@@ -14,7 +14,7 @@ from __future__ import annotations
 from typing import List, Sequence
 
 from .._native import native
-from .token_step import KVCache, kv_cache, kv_cache_read, kv_cache_write, qk_norm_rope  # noqa: F401
+from .token_step import KVCache, kv_cache, kv_cache_read, kv_cache_write, lora_add, paged_attention, qk_norm_rope  # noqa: F401
 
 
 def _k():

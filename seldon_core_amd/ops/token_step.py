@@ -22,6 +22,7 @@ Kernel sources: csrc/kernels/{rope,kv_cache,paged_attention,lora}.hip.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 from .._native import native
@@ -242,6 +243,130 @@ def kv_cache_read(cache: KVCache, slots, dtype=None) -> Tuple:
     return k, v
 
 
+# --------------------------------------------------------------- attention
+_workspace = None
+
+
+def _attention_workspace(*sizes):
+    """fp32 numbers of workspace for (batch, kv heads, group, dim, tokens, window)."""
+    global _workspace
+    if _workspace is None:
+        _workspace = functools.lru_cache(maxsize=1024)(_k().paged_attention_workspace)
+    return _workspace(*sizes)
+
+
+def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[float] = None, window: int = 0,
+                    return_lse: bool = False, out=None):
+    """Attention of one new token per request over its tokens in a paged cache.
+
+    ``q`` [B, Hq, D] (fp16 or bf16, any strides but a contiguous last
+    dimension); the ``cache`` is of q's type, float8_e4m3fn or int8, and query
+    head h reads its head h // (Hq / H).  ``page_table`` [B, W] int32 (rows may
+    be strided) names each request's pages in order, ``lengths`` [B] int32 how
+    many tokens it has, its new one among them: that one sees all of them, or
+    the last ``window``.  ``scale`` is D ** -0.5 unless given.
+
+    D is at most 256 and a row of the cache a multiple of 16 bytes (D a multiple
+    of 8, of 16 with 8 bits), starting at one.  A length beyond the table counts
+    as the table's end, a negative one as 0; tokens on a page outside the cache
+    are left out, and what the cache holds where nothing is seen (anything, NaN
+    too) does not matter.  A request that sees nothing gets zeros.
+
+    Returns [B, Hq, D] in q's type (``out`` if given: contiguous, not
+    overlapping q), with ``return_lse`` also the natural logsumexp of its scores
+    [B, Hq] in fp32, -inf where nothing is seen.
+    """
+    _tensor(q, "q", 3, (torch.bfloat16, torch.float16))
+    dev = q.device
+    c, ptrs, cst = _cache(cache, dev)
+    B, Hq, D = q.shape
+    pages, page, H, dim = c.shape
+    if c.dtype.itemsize != 1 and c.dtype != q.dtype:
+        raise TypeError(f"a cache of {c.dtype} does not go with queries of {q.dtype}")
+    if dim != D or Hq % H or not Hq:
+        raise ValueError(f"queries {tuple(q.shape)} do not go with a cache of {H} heads of {dim}")
+    if D > 256 or D * c.dtype.itemsize % 16:
+        raise ValueError(f"dim must be at most 256 and fill multiples of 16 bytes in the cache, got {D} of {c.dtype}")
+    _tensor(page_table, "page_table", 2, (torch.int32,), dev)
+    _tensor(lengths, "lengths", 1, (torch.int32,), dev, contiguous=True)
+    W = page_table.shape[1]
+    if page_table.shape[0] != B or lengths.shape[0] != B:
+        raise ValueError(f"page_table {tuple(page_table.shape)} and lengths {tuple(lengths.shape)} must have {B} rows")
+    if W < 1 or W * page > 1 << 30:
+        raise ValueError(f"page_table holds {W * page} tokens for a request: at least 1, at most 2^30")
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+    else:
+        _tensor(out, "out", 3, (q.dtype,), dev, contiguous=True)
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    if B:
+        n = _attention_workspace(B, H, Hq // H, D, W * page, window)
+        ws = torch.empty(n, dtype=torch.float32, device=dev)
+        _launch(q, _k().paged_attention, q.data_ptr(), q.stride(0), q.stride(1), _TYPE[q.dtype], ptrs, cst, _TYPE[c.dtype],
+                pages, page, page_table.data_ptr(), page_table.stride(0), W, lengths.data_ptr(), B, H, Hq // H, D, window,
+                D ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), n)
+    return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------- adapters
+_lora_workspace = None
+
+
+def lora_add(y, x, A, B, adapters, scales=None, out=None):
+    """``y + scales[a] * (x @ A[a].T) @ B[a].T`` with the adapter ``a`` of each
+    row: low-rank adapters of many requests at once beside the projection whose
+    output ``y`` is.
+
+    ``x`` [T, K] and ``y`` [T, M] (fp32, fp16 or bf16, all of one type; rows may
+    be strided, such as a part of a fused projection); ``A`` [N, r, K] and ``B``
+    [N, M, r], contiguous, r at most 128 (pad a smaller rank with zeros);
+    ``adapters`` [T] int32 or int64; ``scales`` [N] fp32.  A row whose adapter is
+    negative or behind the last keeps y.  Rows may come in any order; many rows
+    are fastest where those of one adapter lie together.
+
+    Sums are fp32, with one rounding at the end.  Returns a new tensor, or
+    ``out``, which may be ``y`` itself (other overlaps are not allowed).
+    """
+    global _lora_workspace
+    _tensor(y, "y", 2, _FLOATS)
+    dev, dt = y.device, y.dtype
+    _tensor(x, "x", 2, (dt,), dev)
+    _tensor(A, "A", 3, (dt,), dev, contiguous=True)
+    _tensor(B, "B", 3, (dt,), dev, contiguous=True)
+    T, M = y.shape
+    N, r, K = A.shape
+    if x.shape != (T, K) or B.shape != (N, M, r):
+        raise ValueError(f"x {tuple(x.shape)}, y {tuple(y.shape)}, A {tuple(A.shape)} and B {tuple(B.shape)} do not go together")
+    if not 1 <= r <= 128 or not 1 <= K <= 1 << 24 or M > 1 << 24 or not N:
+        raise ValueError(f"rank must be 1 to 128 and there must be an adapter, got A {tuple(A.shape)}")
+    _tensor(adapters, "adapters", 1, _INDEX, dev, contiguous=True)
+    if adapters.shape[0] != T:
+        raise ValueError(f"adapters must have {T} values, got {adapters.shape[0]}")
+    if scales is not None:
+        _tensor(scales, "scales", 1, (torch.float32,), dev, contiguous=True)
+        if scales.shape[0] != N:
+            raise ValueError(f"scales must have {N} values, got {scales.shape[0]}")
+    if out is None:
+        out = torch.empty((T, M), dtype=dt, device=dev)
+    else:
+        _tensor(out, "out", 2, (dt,), dev)
+        if out.shape != y.shape:
+            raise ValueError(f"out must be {tuple(y.shape)}, got {tuple(out.shape)}")
+    if T and M:
+        if _lora_workspace is None:
+            _lora_workspace = functools.lru_cache(maxsize=1024)(_k().lora_workspace)
+        n = _lora_workspace(T, K, r)
+        ws = torch.empty(n, dtype=torch.float32, device=dev)
+        _launch(y, _k().lora_add, y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0),
+                A.data_ptr(), B.data_ptr(), adapters.data_ptr(), _INDEX[adapters.dtype],
+                0 if scales is None else scales.data_ptr(), T, K, M, r, N, _TYPE[dt], ws.data_ptr(), n)
+    return out
+
+
 # ------------------------------------------------------------ CPU references
 def qk_norm_rope_ref(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
     """64-bit reference of :func:`qk_norm_rope` on any device."""
@@ -279,3 +404,46 @@ def kv_quantise_ref(x, dtype):
     if dtype == torch.float8_e4m3fn:
         return y.to(dtype), scale
     return torch.nan_to_num(y).round().clamp(-127, 127).to(torch.int8), scale
+
+
+def paged_attention_ref(q, cache, page_table, lengths, scale=None, window=0):
+    """64-bit reference of :func:`paged_attention` -> (out, lse, sum of |weight * value|)."""
+    B, Hq, D = q.shape
+    pages, page, H, _ = cache.k.shape
+    g = Hq // H
+    scale = D ** -0.5 if scale is None else scale
+    out, mag = (torch.zeros((B, Hq, D), dtype=torch.float64) for _ in range(2))
+    lse = torch.full((B, Hq), float("-inf"), dtype=torch.float64)
+
+    def rows(x, s, p, at):
+        y = x[p, at].float().double() if s is not None else x[p, at].double()
+        return y if s is None else y * s[p, at].double()[..., None]
+
+    for b in range(B):
+        n = min(max(int(lengths[b]), 0), page_table.shape[1] * page)
+        t = torch.arange(max(0, n - window) if window else 0, n)
+        p = page_table[b][t // page].long()
+        keep = (p >= 0) & (p < pages)
+        t, p = t[keep], p[keep]
+        if not len(t):
+            continue
+        k, v = rows(cache.k, cache.k_scales, p, t % page), rows(cache.v, cache.v_scales, p, t % page)
+        for h in range(Hq):
+            s = k[:, h // g] @ q[b, h].double() * scale
+            lse[b, h] = torch.logsumexp(s, 0)
+            w = torch.softmax(s, 0)
+            out[b, h], mag[b, h] = w @ v[:, h // g], w @ v[:, h // g].abs()
+    return out, lse, mag
+
+
+def lora_add_ref(y, x, A, B, adapters, scales=None):
+    """64-bit reference of :func:`lora_add` -> (out, sum of |x||A||B| as a measure of its rounding)."""
+    out = y.double().clone()
+    mag = torch.zeros_like(out)
+    for a in range(A.shape[0]):
+        rows = (adapters == a).nonzero()[:, 0]
+        s = 1.0 if scales is None else scales[a].double()
+        Aa, Ba, xa = A[a].double(), B[a].double(), x[rows].double()
+        out[rows] += s * ((xa @ Aa.T) @ Ba.T)
+        mag[rows] = abs(s) * ((xa.abs() @ Aa.abs().T) @ Ba.abs().T)
+    return out, mag

@@ -29,11 +29,12 @@ def randn(g, *shape, dtype=torch.float32):
 
 
 def close(got, ref, dtype, atol):
-    """|got - ref| <= u |ref| + atol everywhere; atol may be a tensor."""
+    """|got - ref| <= u |ref| + atol everywhere (atol may be a tensor), and NaN exactly where the reference has it."""
     got, ref = got.double().cpu(), ref.double().cpu()
     over = (got - ref).abs() - (u(dtype) * ref.abs() + atol)
-    assert torch.isfinite(got).all()
-    assert float(over.max()) <= 0, f"over the tolerance by {float(over.max()):.3e}"
+    assert torch.equal(got.isnan(), ref.isnan()) and not got.isinf().any()
+    over = over[~ref.isnan()]
+    assert not len(over) or float(over.max()) <= 0, f"over the tolerance by {float(over.max()):.3e}"
 
 
 # ------------------------------------------------------- norm and rotation
@@ -221,3 +222,240 @@ def test_kv_cache_layouts_and_far_offsets():
     assert torch.equal(c.k[-1, -1], k[1]) and torch.equal(c.v[1_100_000 // page, 1_100_000 % page], v[3])
     kr, vr = ops.kv_cache_read(c, slots)
     assert torch.equal(kr, k) and torch.equal(vr, v)
+
+
+# --------------------------------------------------------------- attention
+def attention_inputs(g, lens, Hq, H, D, page, dtype, cache, spare=3, sharp=2.0, heads_first=False):
+    """A pool with NaN wherever no request has a token, and a table with -1 behind each request's pages."""
+    need = [-(-max(n, 0) // page) for n in lens]
+    pages = sum(need) + spare
+    W = max(1, max(need))
+    perm = torch.randperm(pages, generator=g)
+    table = torch.full((len(lens), W), -1, dtype=torch.int32)
+    at = 0
+    used = torch.zeros((pages, page), dtype=torch.bool)
+    for b, n in enumerate(lens):
+        table[b, :need[b]] = perm[at:at + need[b]].int()
+        at += need[b]
+        t = torch.arange(max(n, 0))
+        used[table[b, t // page].long(), t % page] = True
+    kv = []
+    for _ in range(2):
+        x = randn(g, pages, page, H, D, dtype=dtype)
+        if cache == "same":
+            x[~used] = math.nan
+            kv.append((x, None))
+        else:
+            codes, scales = ops.token_step.kv_quantise_ref(x, E4M3 if cache == "e4m3" else torch.int8)
+            scales[~used] = math.nan
+            if cache == "e4m3":
+                codes.view(torch.uint8)[~used] = 0x7f  # NaN
+            kv.append((codes, scales))
+    q = (randn(g, len(lens), Hq, D) * sharp).to(dtype)
+    c = ops.KVCache(kv[0][0], kv[1][0], kv[0][1], kv[1][1])
+    return q, c, table, torch.tensor(lens, dtype=torch.int32)
+
+
+def to_gpu(c, heads_first=False):
+    if heads_first:  # the pages of a head together
+        return ops.KVCache(*(None if x is None else x.transpose(1, 2).contiguous().cuda().transpose(1, 2) for x in c))
+    return ops.KVCache(*(None if x is None else x.cuda() for x in c))
+
+
+def attention_check(got, lse, q, c, table, lens, scale=None, window=0):
+    ref, rlse, mag = ops.token_step.paged_attention_ref(q, c, table, lens, scale, window)
+    D = q.shape[-1]
+    n = min(int(lens.clamp_min(0).max()), table.shape[1] * c.k.shape[1]) + 1
+    sc = D ** -0.5 if scale is None else abs(scale)
+    k = c.k.double() if c.k_scales is None else c.k.float().double() * c.k_scales.double()[..., None]
+    # |s| and the sum of |q||k| by Cauchy and Schwarz; an fp32 sum of D products is off by at most (D + 3) 2^-24 of that, and
+    # as much again enters through the softmax's total.  The sum over n tokens adds n 2^-24, exp2 and the joins under 64 * 2^-24,
+    # the split weights 2^-16.  All of it relative to the sum of |weight * value|.
+    s = sc * float(q.double().norm(dim=-1).max()) * float(torch.nan_to_num(k, posinf=0.0, neginf=0.0).norm(dim=-1).max())
+    rel = (2 * (D + 3) * s + n + 64) * 2.0 ** -24 + 2.0 ** -16
+    close(got, ref, q.dtype, rel * mag)
+    if lse is not None:
+        lse = lse.cpu().double()
+        seen = torch.isfinite(rlse)
+        assert torch.equal(lse.isnan(), rlse.isnan()) and torch.equal(lse == -math.inf, rlse == -math.inf)
+        assert bool(((lse - rlse)[seen].abs() <= ((D + 3) * s + n + 64) * 2.0 ** -24 + rlse[seen].abs() * 2.0 ** -22).all())
+    return ref
+
+
+ATTENTION = [  # lengths, query heads, key heads, dim, page, window
+    ([1], 1, 1, 64, 16, 0), ([0], 4, 2, 128, 16, 0), ([5, 0, 1], 8, 2, 128, 16, 0), ([128, 127, 129, 31, 32, 33], 4, 4, 64, 24, 0),
+    ([1000, 3, 256, 0, 511], 32, 8, 128, 16, 0), ([700], 7, 1, 128, 64, 0), ([300, 40], 40, 2, 64, 1, 0),
+    ([4097], 16, 1, 256, 32, 0), ([90, 2000], 6, 2, 80, 7, 0), ([1500, 10, 0], 12, 12, 96, 48, 100),
+    ([600, 601, 5], 4, 2, 256, 16, 1), ([2500], 8, 8, 64, 16, 777), ([64] * 37, 8, 4, 128, 16, 0),
+    ([3, 700] * 150, 2, 1, 64, 8, 0), ([140] * 5, 34, 1, 48, 16, 129), ([333], 5, 1, 16, 16, 0), ([50], 3, 3, 208, 5, 60)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", ATTENTION, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{c[1]}-{c[2]}-{c[3]}-{c[4]}-{c[5]}")
+@pytest.mark.parametrize("cache", ["same", "e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_paged_attention(case, cache, dtype):
+    lens, Hq, H, D, page, window = case
+    g = gen(len(lens), *case[1:])
+    q, c, table, lengths = attention_inputs(g, lens, Hq, H, D, page, DT[dtype], cache)
+    got, lse = ops.paged_attention(q.cuda(), to_gpu(c, heads_first=page % 2 == 0), table.cuda(), lengths.cuda(), window=window,
+                                   return_lse=True)
+    attention_check(got, lse, q, c, table, lengths, window=window)
+    assert not got[lengths.cuda() == 0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["same", "int8"])
+def test_paged_attention_bad_pages_lengths_and_strides(cache):
+    g = gen(3, 1)
+    lens = [200, 70, 33, 129, 64]
+    q, c, table, lengths = attention_inputs(g, lens, 8, 2, 128, 16, torch.bfloat16, cache)
+    pages = c.k.shape[0]
+    table[0, 3], table[0, 7], table[1, 0] = pages, -2, 2 ** 31 - 1  # pages that do not exist: their tokens are left out
+    table[2] = -1  # nothing is left of this one
+    lengths[3] = 10 ** 9  # longer than the table: its end, whose last real page holds NaN behind token 129: so does the output
+    lengths[4] = -5  # nothing
+    wide = torch.full((5, table.shape[1] + 3), 10 ** 6, dtype=torch.int32)
+    wide[:, :-3] = table
+    qs = torch.full((5, 8, 3 * 128), math.nan, dtype=torch.bfloat16)
+    qs[:, :, 128:256] = q
+    out = torch.full((5, 8, 128), math.nan, dtype=torch.bfloat16, device="cuda")
+    got, lse = ops.paged_attention(qs.cuda()[:, :, 128:256], to_gpu(c), wide.cuda()[:, :-3], lengths.cuda(), scale=0.25,
+                                   return_lse=True, out=out)
+    assert got is out
+    attention_check(got, lse, q, c, table, lengths, scale=0.25)
+    assert got[3].isnan().all() and not got[0].isnan().any()
+    assert not got[2].any() and not got[4].any()
+    # queries that start at an odd element
+    qo = torch.zeros(q.numel() + 1, dtype=q.dtype, device="cuda")[1:].view(q.shape)
+    qo.copy_(q)
+    again = ops.paged_attention(qo, to_gpu(c), table.cuda(), lengths.cuda(), scale=0.25)
+    assert torch.equal(again.nan_to_num(7.0), got.nan_to_num(7.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_paged_attention_scores_far_apart(dtype):
+    """One token far above a long flat tail, rising and falling scores, and scores of thousands."""
+    g = gen(8)
+    n, D = 5000, 64
+    dt = DT[dtype]
+    for kind in ("peak first", "peak last", "rising", "falling", "huge"):
+        q, c, table, lengths = attention_inputs(g, [n], 2, 1, D, 16, dt, "same", sharp=0.0)
+        q[..., 0] = 8
+        slots = table[0, torch.arange(n) // 16].long() * 16 + torch.arange(n) % 16
+        k = c.k.view(-1, D)
+        k[slots] = 0
+        s = torch.zeros(n)
+        if kind == "peak first":
+            s[3] = 17
+        elif kind == "peak last":
+            s[n - 2] = 17
+        elif kind == "huge":
+            s = torch.randn(n, generator=g) * 3000
+        else:
+            s = torch.linspace(-40, 40, n) * (1 if kind == "rising" else -1)
+        k[slots, 0] = s.to(dt)
+        got, lse = ops.paged_attention(q.cuda(), to_gpu(c), table.cuda(), lengths.cuda(), return_lse=True)
+        attention_check(got, lse, q, c, table, lengths)
+
+
+@pytest.mark.gpu
+def test_paged_attention_pool_past_2_31_elements():
+    g = gen(9)
+    pages, page, H, D = 70000, 32, 8, 128  # 2.3 G elements
+    c = ops.KVCache(*(torch.zeros((pages, page, H, D), dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    n = 300
+    table = torch.tensor([[pages - 1 - 7 * i for i in range(10)]], dtype=torch.int32)
+    t = torch.arange(n)
+    slots = table[0, t // page].long() * page + t % page
+    k, v = (randn(g, n, H, D, dtype=torch.bfloat16) for _ in range(2))
+    ops.kv_cache_write(c, k.cuda(), v.cuda(), slots.cuda())
+    q = randn(g, 1, 16, D, dtype=torch.bfloat16)
+    got = ops.paged_attention(q.cuda(), c, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda())
+    small = ops.KVCache(*(torch.zeros((10, page, H, D), dtype=torch.bfloat16) for _ in range(2)))
+    small.k.view(-1, H, D)[:n], small.v.view(-1, H, D)[:n] = k, v
+    attention_check(got, None, q, small, torch.arange(10, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32))
+
+
+# ---------------------------------------------------------------- adapters
+LORA = [  # rows, inner, outer, rank, adapters, mixed
+    (1, 1, 1, 1, 1, True), (1, 4096, 4096, 16, 4, True), (64, 1024, 640, 16, 32, True), (17, 200, 77, 12, 3, True),
+    (333, 1001, 503, 9, 5, False), (16, 512, 512, 64, 16, True), (40, 300, 1030, 100, 2, False), (5, 4104, 72, 128, 5, True),
+    (1025, 512, 384, 8, 3, False), (1100, 320, 200, 32, 40, True), (2000, 264, 1100, 64, 7, False), (1030, 130, 66, 128, 2, True),
+    (1024, 64, 64, 33, 1000, True), (3, 8200, 64, 5, 2, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", LORA, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("dtype", list(DT))
+def test_lora_add(case, dtype):
+    T, K, M, r, N, mixed = case
+    dt = DT[dtype]
+    g = gen(*case[:5])
+    x, y = randn(g, T, K, dtype=dt), randn(g, T, M, dtype=dt)
+    A, B = (randn(g, N, r, K) * K ** -0.5).to(dt), (randn(g, N, M, r) * r ** -0.5).to(dt)
+    ids = torch.randint(-1, N + 1, (T,), generator=g) if mixed else torch.arange(T) * N // T
+    if T > 3:
+        ids[T // 3] = -7
+    scales = randn(g, N)
+    want, mag = ops.token_step.lora_add_ref(y, x, A, B, ids, scales)
+    yd = y.cuda()
+    got = ops.lora_add(yd, x.cuda(), A.cuda(), B.cuda(), ids.cuda(), scales.cuda())
+    assert torch.equal(yd.cpu(), y)
+    # the two sums in fp32 ((K + r + 8) 2^-24 of the sum of magnitudes), h in two 16-bit parts: 2^-16 of it (bf16), or 2^-24 of the
+    # row's largest h for fp16, whose remainder may be subnormal
+    atol = (K + r + 8) * 2.0 ** -24 * mag + (2.0 ** -16 * mag if dt == torch.bfloat16 else 0)
+    if dt == torch.float16:
+        ok = (ids >= 0) & (ids < N)
+        i = torch.where(ok, ids, 0)
+        for t in range(T):
+            if ok[t]:
+                h = (A[i[t]].double() @ x[t].double()).abs().max() * abs(scales[i[t]].double())
+                atol[t] += 2.0 ** -23 * h * B[i[t]].double().abs().sum(-1)
+    close(got, want, dt, atol + 2.0 ** -24 * want.abs())
+    untouched = (ids < 0) | (ids >= N)
+    assert torch.equal(got.cpu()[untouched], y[untouched])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [6, 1500])
+def test_lora_add_strides_in_place_and_index_types(T):
+    """A part of a fused projection changed in place, and its neighbours left as they were."""
+    g = gen(T)
+    K, M, r, N = 128, 192, 16, 4
+    x, y = randn(g, T, K + 8, dtype=torch.bfloat16), randn(g, T, 3 * M, dtype=torch.bfloat16)
+    A, B = randn(g, N, r, K, dtype=torch.bfloat16) * 0.1, randn(g, N, M, r, dtype=torch.bfloat16)
+    ids = (torch.arange(T) % (N + 1) - 1).int()
+    want, mag = ops.token_step.lora_add_ref(y[:, M:2 * M], x[:, 8:], A, B, ids)
+    for off in (0, 1):  # aligned rows, and rows that no vector fits
+        buf = torch.zeros(T * 3 * M + off, dtype=torch.bfloat16, device="cuda")
+        yd = buf[off:].view(T, 3 * M)
+        yd.copy_(y)
+        part = yd[:, M:2 * M]
+        got = ops.lora_add(part, x.cuda()[:, 8:], A.cuda(), B.cuda(), ids.cuda(), out=part)
+        assert got.data_ptr() == part.data_ptr()
+        close(part, want, torch.bfloat16, (2.0 ** -16 + (K + r + 8) * 2.0 ** -24) * mag + 2.0 ** -24 * want.abs())
+        assert torch.equal(yd.cpu()[:, :M], y[:, :M]) and torch.equal(yd.cpu()[:, 2 * M:], y[:, 2 * M:])
+        assert torch.equal(part.cpu()[ids < 0], y[:, M:2 * M][ids < 0])
+
+
+@pytest.mark.gpu
+def test_lora_add_large_and_infinite_values():
+    """fp16: an h far beyond fp16's range that B brings back; infinities reach only their own rows and columns."""
+    g = gen(77)
+    T, K, M, r = 5, 256, 64, 8
+    x = (randn(g, T, K).abs() * 100 + 100).half()
+    A, B = torch.full((1, r, K), 30.0).half(), (randn(g, 1, M, r) * 1e-4).half()
+    y, ids = randn(g, T, M).half(), torch.zeros(T, dtype=torch.int32)
+    want, mag = ops.token_step.lora_add_ref(y, x, A, B, ids)  # h is about 10^6
+    got = ops.lora_add(y.cuda(), x.cuda(), A.cuda(), B.cuda(), ids.cuda())
+    close(got, want, torch.float16, ((K + r + 8) * 2.0 ** -24 + 2.0 ** -21) * mag + 2.0 ** -24 * want.abs())
+    for dt in (torch.float16, torch.bfloat16, torch.float32):
+        xi = x.to(dt)
+        xi[2, 3] = math.inf
+        got = ops.lora_add(y.to(dt).cuda(), xi.cuda(), A.to(dt).cuda(), B.abs().clamp_min(1e-4).to(dt).cuda(), ids.cuda()).cpu()
+        assert (got[2] == math.inf).all() and torch.isfinite(got[[0, 1, 3, 4]]).all()
+    e = ops.lora_add(torch.empty((0, M), device="cuda"), torch.empty((0, K), device="cuda"), A.float().cuda(), B.float().cuda(),
+                     torch.empty(0, dtype=torch.int32, device="cuda"))
+    assert e.shape == (0, M)

@@ -39,7 +39,7 @@ LIB_SOURCES = [
     "server/http_server.cc", "server/grpc_server.cc", "server/remote_unit.cc",
     "gpu/models.cc", "gpu/batcher.cc", "gpu/driver.cc", "gpu/router.cc", "gpu/graph.cc", "gpu/replica.cc", "gpu/mlp_model.cc", "gpu/lstm_model.cc", "gpu/maha_device.cc", "parallel/fabric.cc", "parallel/mesh.cc",
     "kernels/linear.hip", "kernels/linear_graph.hip", "kernels/tree.hip", "kernels/combine.hip", "kernels/bandit.hip", "kernels/image.hip", "kernels/mlp.hip", "kernels/mahalanobis.hip", "kernels/lstm.hip", "kernels/lstm_valu.hip", "kernels/gemm.hip",
-    "kernels/rope.hip", "kernels/kv_cache.hip",
+    "kernels/rope.hip", "kernels/kv_cache.hip", "kernels/paged_attention.hip", "kernels/lora.hip",
     "bindings/module.cc",
 ]
 LOADGEN_SOURCES = ["tools/loadgen.cc", "core/json.cc"]
