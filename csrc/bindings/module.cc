@@ -1175,11 +1175,11 @@ PYBIND11_MODULE(_C, m) {
       a.scale[i] = P<float>(cache[2 + i]);
       a.s_page[i] = cst[6 + 3 * i], a.s_slot[i] = cst[7 + 3 * i], a.s_head[i] = cst[8 + 3 * i];
     }
-    if (page_size < 1 || page_size > 0x7fffffff) throw std::invalid_argument("kv_cache: page size");
+    if (page_size < 1 || page_size > 0x7fffffff || heads < 1) throw std::invalid_argument("kv_cache: sizes");
     a.type = type, a.cache_type = cache_type;
     a.slots = P<const void>(slots), a.slots64 = slots64;
     a.page = kern::FastDiv(uint32_t(page_size)), a.slots_total = pages * page_size;
-    a.rows = rows, a.heads = heads, a.dim = dim;
+    a.rows = rows, a.heads = kern::FastDiv(uint32_t(heads)), a.dim = dim;
     return a;
   };
   k.def("kv_cache_write", [kv_args](const std::array<uintptr_t, 2>& x, const std::array<int64_t, 4>& xst, int type,
@@ -1207,7 +1207,6 @@ PYBIND11_MODULE(_C, m) {
       throw std::invalid_argument("paged_attention: sizes");
     kern::PagedAttentionArgs a;
     a.q = P<const void>(q), a.q_batch = q_batch, a.q_head = q_head, a.type = type;
-    a.q_vector = q % 16 == 0 && q_batch % 8 == 0 && q_head % 8 == 0;
     for (size_t i = 0; i < 2; ++i) {
       a.cache[i] = P<const void>(cache[i]);
       a.c_page[i] = cst[3 * i], a.c_slot[i] = cst[3 * i + 1], a.c_head[i] = cst[3 * i + 2];

@@ -20,22 +20,29 @@ struct e4m3 {
 
 template <class T> constexpr bool kQuantised = sizeof(T) == 1;
 
-// V consecutive elements as fp32.  The pointer is aligned to
-// min(16, V * sizeof(T)) bytes: one vector load for each 16 bytes.
+// U at any address: the hardware's vector loads and stores need no alignment (a run
+// across a cache line costs a second access, far less than one access an element).
+template <class U> __device__ __forceinline__ U load_any(const void* p) {
+  U u;
+  __builtin_memcpy(&u, p, sizeof(U));
+  return u;
+}
+template <class U> __device__ __forceinline__ void store_any(void* p, const U& u) { __builtin_memcpy(p, &u, sizeof(U)); }
+
+// V consecutive elements as fp32, from any address, 16 bytes at most a load.
 template <int V, class T> __device__ __forceinline__ void load_run(const T* p, float* f) {
   if constexpr (std::is_same_v<T, e4m3>) {
     if constexpr (V % 4 == 0) {
-      using U = uint32_t __attribute__((ext_vector_type(V / 4)));
-      const U u = *reinterpret_cast<const U*>(p);
+      struct Words {
+        uint32_t w[V / 4];
+      };
+      const Words u = load_any<Words>(p);
 #pragma unroll
       for (int i = 0; i < V / 4; ++i) {
-        uint32_t w;
-        if constexpr (V == 4) w = *reinterpret_cast<const uint32_t*>(&u);
-        else w = u[i];
-        f[4 * i + 0] = __builtin_amdgcn_cvt_f32_fp8(int(w), 0);
-        f[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(int(w), 1);
-        f[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(int(w), 2);
-        f[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(int(w), 3);
+        f[4 * i + 0] = __builtin_amdgcn_cvt_f32_fp8(int(u.w[i]), 0);
+        f[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(int(u.w[i]), 1);
+        f[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(int(u.w[i]), 2);
+        f[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(int(u.w[i]), 3);
       }
     } else {
 #pragma unroll
@@ -49,7 +56,7 @@ template <int V, class T> __device__ __forceinline__ void load_run(const T* p, f
       if constexpr (N == 1) {
         f[j] = float(p[j]);
       } else {
-        const U u = *reinterpret_cast<const U*>(p + j);
+        const U u = load_any<U>(p + j);
 #pragma unroll
         for (int i = 0; i < N; ++i) f[j + i] = float(u[i]);
       }
@@ -62,18 +69,16 @@ template <int V, class T> __device__ __forceinline__ void load_run(const T* p, f
 template <int V, class T> __device__ __forceinline__ void store_run(T* p, const float* f) {
   if constexpr (std::is_same_v<T, e4m3>) {
     if constexpr (V % 4 == 0) {
+      struct Words {
+        uint32_t w[V / 4];
+      } u;
 #pragma unroll
-      for (int i = 0; i < V; i += 8) {
-        uint32_t w[2];
-#pragma unroll
-        for (int j = 0; j < 2 && i + 4 * j < V; ++j) {
-          int u = __builtin_amdgcn_cvt_pk_fp8_f32(f[i + 4 * j], f[i + 4 * j + 1], 0, false);
-          u = __builtin_amdgcn_cvt_pk_fp8_f32(f[i + 4 * j + 2], f[i + 4 * j + 3], u, true);
-          w[j] = uint32_t(u);
-        }
-        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-        else *reinterpret_cast<uint2*>(p + i) = make_uint2(w[0], w[1]);
+      for (int i = 0; i < V / 4; ++i) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], w, true);
+        u.w[i] = uint32_t(w);
       }
+      store_any(p, u);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) p[i].bits = uint8_t(__builtin_amdgcn_cvt_pk_fp8_f32(f[i], 0.f, 0, false) & 0xff);
@@ -89,7 +94,7 @@ template <int V, class T> __device__ __forceinline__ void store_run(T* p, const 
         U u;
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = T(f[j + i]);
-        *reinterpret_cast<U*>(p + j) = u;
+        store_any(p + j, u);
       }
     }
   }

@@ -14,8 +14,7 @@
 //
 // Both kernels are bound by memory and touch every byte once.  A (row, head)
 // belongs to a group of lanes, 8 values a lane (16 bytes of a 16-bit type); the
-// largest magnitude is taken in registers over the group.  k and v go through
-// one launch, as the two halves of the grid's y.
+// largest magnitude is taken in registers over the group.
 #include <hip/hip_runtime.h>
 
 #include <stdexcept>
@@ -45,124 +44,144 @@ template <class C> __device__ __forceinline__ float head_scale(float top) {
 }
 
 template <class C, int V> __device__ __forceinline__ void encode(float* f, float scale) {
+  const float inv = 1.f / scale;
+  if constexpr (std::is_same_v<C, e4m3>) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if constexpr (std::is_same_v<C, e4m3>) {
-      f[i] *= 1.f / scale;  // a power of two: exact
-    } else {
-      f[i] /= scale;  // correctly rounded, so the codes are those of any correct division
-      f[i] = f[i] == f[i] ? fminf(fmaxf(rintf(f[i]), -127.f), 127.f) : 0.f;
+    for (int i = 0; i < V; ++i) f[i] *= inv;  // a power of two: exact
+  } else {
+    // The code is the correctly rounded quotient's nearest whole number.  x * inv is within 2^-16 of that quotient
+    // (|x / scale| <= 127, three roundings), so only next to a half can the two differ: there it is divided.  A
+    // division for each value made the kernel twice as slow as its memory (about 14 instructions each).
+    float n[V], border = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float q = f[i] * inv;
+      n[i] = rintf(q);
+      border = fmaxf(border, fabsf(q - n[i]));
     }
+    if (border > 0.5f - 0x1p-14f) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) n[i] = rintf(f[i] / scale);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = n[i] == n[i] ? fminf(fmaxf(n[i], -127.f), 127.f) : 0.f;
   }
 }
 
-// X: the rows' type, C: the cache's.
+// The place of a row's slot in the cache.
+struct Place {
+  bool in;
+  uint32_t page, at;
+  __device__ __forceinline__ Place(const KvCacheArgs& a, int64_t row) {
+    const int64_t slot = load_index(a.slots, a.slots64, row);
+    in = slot >= 0 && slot < a.slots_total;
+    page = in ? a.page.div(uint32_t(slot)) : 0;
+    at = in ? uint32_t(slot) - page * a.page.d : 0;
+  }
+};
+
+// X: the rows' type, C: the cache's.  A group of lanes takes k and v of its head
+// one behind the other, so both are under way at once and share the slot's place.
 template <class X, class C, int V>
-__global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(const KvCacheArgs a, int lanes) {
-  const int which = blockIdx.y;
-  const int64_t item = int64_t(blockIdx.x) * (kThreads / lanes) + threadIdx.x / lanes;
+__global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(const KvCacheArgs a, int lanes, int lanes_log2) {
+  const uint32_t item = blockIdx.x * uint32_t(kThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   const int lane = threadIdx.x & (lanes - 1);
-  if (item >= a.rows * a.heads) return;
-  const int64_t row = item / a.heads;
-  const int head = int(item - row * a.heads);
-  const int64_t slot = load_index(a.slots, a.slots64, row);
-  if (slot < 0 || slot >= a.slots_total) return;
-  const uint32_t page = a.page.div(uint32_t(slot)), at = uint32_t(slot) - page * a.page.d;
-  const X* const x = static_cast<const X*>(a.x[which]) + row * a.x_row[which] + head * a.x_head[which];
-  C* const c = static_cast<C*>(a.cache[which]) + page * a.c_page[which] + at * a.c_slot[which] + head * a.c_head[which];
+  if (item >= uint32_t(a.rows) * a.heads.d) return;
+  const uint32_t in_row = a.heads.div(item), head = item - in_row * a.heads.d;
+  const int64_t row = in_row;
   constexpr int NS = V == 1 ? 8 : 1;  // dim <= 512
-  float f[NS][V];
-  float top = 0.f;
+  float f[2][NS][V];
 #pragma unroll
-  for (int k = 0; k < NS; ++k) {
-    const int d = (k * lanes + lane) * V;
-    if (d < a.dim) {
-      load_run<V>(x + d, f[k]);
-      if constexpr (kQuantised<C>) {
+  for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float m = fabsf(f[k][i]);
-          top = (m > top || m != m) ? m : top;
+    for (int k = 0; k < NS; ++k) {
+      const int d = (k * lanes + lane) * V;
+      if (d < a.dim) load_run<V>(static_cast<const X*>(a.x[w]) + row * a.x_row[w] + head * a.x_head[w] + d, f[w][k]);
+    }
+  const Place p(a, row);
+  if (!p.in) return;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    C* const c = static_cast<C*>(a.cache[w]) + p.page * a.c_page[w] + p.at * a.c_slot[w] + head * a.c_head[w];
+    float scale = 1.f;
+    if constexpr (kQuantised<C>) {
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < NS; ++k)
+        if ((k * lanes + lane) * V < a.dim) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float m = fabsf(f[w][k][i]);
+            top = (m > top || m != m) ? m : top;
+          }
         }
+      scale = head_scale<C>(group_max(top, lanes));
+      if (lane == 0) a.scale[w][p.page * a.s_page[w] + p.at * a.s_slot[w] + head * a.s_head[w]] = scale;
+    }
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      const int d = (k * lanes + lane) * V;
+      if (d < a.dim) {
+        if constexpr (kQuantised<C>) encode<C, V>(f[w][k], scale);
+        store_run<V>(c + d, f[w][k]);
       }
     }
   }
-  float scale = 1.f;
-  if constexpr (kQuantised<C>) {
-    scale = head_scale<C>(group_max(top, lanes));
-    if (lane == 0)
-      a.scale[which][page * a.s_page[which] + at * a.s_slot[which] + head * a.s_head[which]] = scale;
-  }
-#pragma unroll
-  for (int k = 0; k < NS; ++k) {
-    const int d = (k * lanes + lane) * V;
-    if (d < a.dim) {
-      if constexpr (kQuantised<C>) encode<C, V>(f[k], scale);
-      store_run<V>(c + d, f[k]);
-    }
-  }
 }
 
 template <class X, class C, int V>
-__global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(const KvCacheArgs a, int lanes) {
-  const int which = blockIdx.y;
-  const int64_t item = int64_t(blockIdx.x) * (kThreads / lanes) + threadIdx.x / lanes;
+__global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(const KvCacheArgs a, int lanes, int lanes_log2) {
+  const uint32_t item = blockIdx.x * uint32_t(kThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   const int lane = threadIdx.x & (lanes - 1);
-  if (item >= a.rows * a.heads) return;
-  const int64_t row = item / a.heads;
-  const int head = int(item - row * a.heads);
-  const int64_t slot = load_index(a.slots, a.slots64, row);
-  const bool in = slot >= 0 && slot < a.slots_total;
-  const uint32_t page = in ? a.page.div(uint32_t(slot)) : 0, at = in ? uint32_t(slot) - page * a.page.d : 0;
-  X* const x = static_cast<X*>(a.x[which]) + row * a.x_row[which] + head * a.x_head[which];
-  const C* const c =
-      static_cast<const C*>(a.cache[which]) + page * a.c_page[which] + at * a.c_slot[which] + head * a.c_head[which];
-  float scale = 1.f;
-  if constexpr (kQuantised<C>) {
-    if (in) scale = a.scale[which][page * a.s_page[which] + at * a.s_slot[which] + head * a.s_head[which]];
-  }
+  if (item >= uint32_t(a.rows) * a.heads.d) return;
+  const uint32_t in_row = a.heads.div(item), head = item - in_row * a.heads.d;
+  const int64_t row = in_row;
+  const Place p(a, row);
   constexpr int NS = V == 1 ? 8 : 1;
+  float f[2][NS][V], scale[2] = {1.f, 1.f};
 #pragma unroll
-  for (int k = 0; k < NS; ++k) {
-    const int d = (k * lanes + lane) * V;
-    if (d < a.dim) {
-      float f[V];
+  for (int w = 0; w < 2; ++w) {
+    const C* const c = static_cast<const C*>(a.cache[w]) + p.page * a.c_page[w] + p.at * a.c_slot[w] + head * a.c_head[w];
+    if constexpr (kQuantised<C>) {
+      if (p.in) scale[w] = a.scale[w][p.page * a.s_page[w] + p.at * a.s_slot[w] + head * a.s_head[w]];
+    }
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = 0.f;
-      if (in) {
-        load_run<V>(c + d, f);
+    for (int k = 0; k < NS; ++k) {
+      const int d = (k * lanes + lane) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[w][k][i] = 0.f;
+      if (p.in && d < a.dim) load_run<V>(c + d, f[w][k]);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    X* const x = static_cast<X*>(a.x[w]) + row * a.x_row[w] + head * a.x_head[w];
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      const int d = (k * lanes + lane) * V;
+      if (d < a.dim) {
         if constexpr (kQuantised<C>) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) f[i] *= scale;
+          for (int i = 0; i < V; ++i) f[w][k][i] *= scale[w];
         }
+        store_run<V>(x + d, f[w][k]);
       }
-      store_run<V>(x + d, f);
     }
   }
 }
 
 template <class X, class C, int V> void launch(const KvCacheArgs& a, bool write, hipStream_t s) {
-  int lanes = 1;
-  while (lanes < 64 && lanes * V < a.dim) lanes *= 2;
-  const int64_t per = kThreads / lanes, blocks = (a.rows * a.heads + per - 1) / per;
-  if (blocks > 0x7fffffff) throw std::invalid_argument("kv_cache: too many rows for one call");
-  const dim3 grid(unsigned(blocks), 2);
-  if (write) launch_kernel(kv_cache_write_kernel<X, C, V>, grid, kThreads, 0, s, a, lanes);
-  else launch_kernel(kv_cache_read_kernel<X, C, V>, grid, kThreads, 0, s, a, lanes);
+  int lanes = 1, log2 = 0;
+  while (lanes < 64 && lanes * V < a.dim) lanes *= 2, ++log2;
+  const int64_t per = kThreads / lanes, blocks = (a.rows * a.heads.d + per - 1) / per;
+  const dim3 grid{unsigned(blocks)};
+  if (write) launch_kernel(kv_cache_write_kernel<X, C, V>, grid, kThreads, 0, s, a, lanes, log2);
+  else launch_kernel(kv_cache_read_kernel<X, C, V>, grid, kThreads, 0, s, a, lanes, log2);
 }
 
 template <class X, class C> void dispatch(const KvCacheArgs& a, bool write, hipStream_t s) {
-  // runs of 8 values where every row starts at a multiple of them, else one by one
-  int64_t xs = a.dim, cs = a.dim;
-  int64_t xb = 0, cb = 0;
-  for (int i = 0; i < 2; ++i) {
-    xs |= a.x_row[i] | a.x_head[i];
-    cs |= a.c_page[i] | a.c_slot[i] | a.c_head[i];
-    xb |= int64_t(reinterpret_cast<uintptr_t>(a.x[i]));
-    cb |= int64_t(reinterpret_cast<uintptr_t>(a.cache[i]));
-  }
-  const int64_t cw = 8 * sizeof(C) < 16 ? 8 * sizeof(C) : 16;
-  if ((xs | cs) % 8 == 0 && xb % 16 == 0 && cb % cw == 0) return launch<X, C, 8>(a, write, s);
+  // runs of 8 values where rows are made of them, else one by one
+  if (a.dim % 8 == 0) return launch<X, C, 8>(a, write, s);
   return launch<X, C, 1>(a, write, s);
 }
 
@@ -183,7 +202,8 @@ void run(const KvCacheArgs& a, bool write, hipStream_t s) {
     throw std::invalid_argument("kv_cache: at most 2^31 - 1 slots, in pages of at least one");
   if ((a.cache_type == kE4M3 || a.cache_type == kI8) && (!a.scale[0] || !a.scale[1]))
     throw std::invalid_argument("kv_cache: an 8-bit cache has scales");
-  if (a.rows <= 0 || a.heads <= 0) return;
+  if (a.rows <= 0) return;
+  if (a.rows > 0x7fffffff / int64_t(a.heads.d)) throw std::invalid_argument("kv_cache: at most 2^31 - 1 rows times heads");
   switch (a.type) {
     case kF32: return by_cache<float>(a, write, s);
     case kF16: return by_cache<f16>(a, write, s);

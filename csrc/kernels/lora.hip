@@ -31,7 +31,9 @@
 namespace sca::kern {
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4;
+// Waves of a workgroup of NC row tiles: one for each group of a mixed batch's 16
+// rows (8 where the registers of a high rank allow no more), four for a prompt's.
+template <int NR, int NC> constexpr int kWaves = NC > 1 ? 4 : NR <= 2 ? 16 : 8;
 
 using f32x4 = float __attribute__((ext_vector_type(4)));
 template <class T> constexpr int kRun = 16 / int(sizeof(T));   // elements of a lane's 16 bytes
@@ -51,15 +53,14 @@ __device__ __forceinline__ f32x4 mma(frag<float> a, frag<float> b, f32x4 c) {
   return c;
 }
 
-// kRun elements from p[at], zeros from `end` on.  VEC: rows start at multiples of
-// 16 bytes and `end` is a multiple of kRun.
-template <class T, bool VEC> __device__ __forceinline__ frag<T> load_frag(const T* p, int at, int end) {
+// kRun elements from p[at], zeros from `end` on.  EVEN: `end` is a multiple of kRun.
+template <class T, bool EVEN> __device__ __forceinline__ frag<T> load_frag(const T* p, int at, int end) {
   frag<T> x = {};
-  if constexpr (VEC) {
-    if (at < end) x = *reinterpret_cast<const frag<T>*>(p + at);
-  } else {
+  if (at + (EVEN ? 0 : kRun<T> - 1) < end) {
+    x = load_any<frag<T>>(p + at);
+  } else if (!EVEN && at < end) {
 #pragma unroll
-    for (int j = 0; j < kRun<T>; ++j)
+    for (int j = 0; j < kRun<T> - 1; ++j)
       if (at + j < end) x[j] = p[at + j];
   }
   return x;
@@ -103,20 +104,24 @@ __device__ __forceinline__ int set_bits(uint64_t mask, int lane) {
   return __builtin_amdgcn_ds_permute((mine ? rank : behind) * 4, lane);
 }
 
-// How the four waves share `n` groups: over 1, 2 or 4 of them.
-__device__ __forceinline__ int share(int n) { return n >= 3 ? 4 : n == 2 ? 2 : 1; }
+// How `waves` (a power of two) share n groups: over as many of them as there are groups, up to the next power of two.
+__device__ __forceinline__ int share(int n, int waves) {
+  int over = 1;
+  while (over < n && over < waves) over *= 2;
+  return over;
+}
 
 // ---- h[split][row][rank] = sum over the split's part of the inner dimension
 // NR: rank tiles of 16, NC: row tiles of 16.
-template <class T, bool VEC, int NR, int NC>
-__global__ __launch_bounds__(kThreads) void lora_down(const LoraArgs a) {
-  extern __shared__ __attribute__((aligned(16))) float part[];  // [kWaves][16 NC][16 NR + 4]
-  constexpr int kRows = 16 * NC, kRow = 16 * NR + 4;
-  constexpr int kAhead = NR * NC >= 16 ? 2 : NR * NC >= 4 ? 4 : 8;  // steps whose loads are issued together
+template <class T, bool EVEN, int NR, int NC>
+__global__ __launch_bounds__((64 * kWaves<NR, NC>)) void lora_down(const LoraArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][16 NC][16 NR + 4]
+  constexpr int kW = kWaves<NR, NC>, kThreads = 64 * kW, kRows = 16 * NC, kRow = 16 * NR + 4;
+  constexpr int kAhead = NR * NC >= 16 ? 2 : NR * NC >= 2 ? 4 : 8;  // steps whose loads are issued together
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
   const int64_t row0 = int64_t(blockIdx.x) * kRows;
   Groups groups(a, row0, kRows, lane);
-  const int over = share(groups.count()), parts = kWaves / over;
+  const int over = share(groups.count(), kW), parts = kW / over;
   const int my_part = wave / over;
   // steps of kDeep: first those of the split, then those of this wave in it
   const int steps = (a.inner + kDeep<T> - 1) / kDeep<T>;
@@ -152,10 +157,10 @@ __global__ __launch_bounds__(kThreads) void lora_down(const LoraArgs a) {
       for (int j = 0; j < kAhead; ++j) {
         const int k = (s + j) * kDeep<T> + g4 * kRun<T>, end = s + j < w1 ? a.inner : 0;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) af[j][r] = load_frag<T, VEC>(Ar[r], k, end);
+        for (int r = 0; r < NR; ++r) af[j][r] = load_frag<T, EVEN>(Ar[r], k, end);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-          if (c < tiles) xf[j][c] = load_frag<T, VEC>(xr[c], k, end);
+          if (c < tiles) xf[j][c] = load_frag<T, EVEN>(xr[c], k, end);
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
@@ -190,10 +195,9 @@ __global__ __launch_bounds__(kThreads) void lora_down(const LoraArgs a) {
 }
 
 // ---- out = y + B h.  KS: steps of the rank, NC: row tiles of 16.
-// VEC: B's rows, as load_frag has them; the rows of y and out go by a.vector.
-template <class T, bool VEC, int KS, int NC>
-__global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks) {
-  constexpr int kRows = 16 * NC, kDepth = KS * kDeep<T>, kRow = kDepth + kRun<T>;
+template <class T, bool EVEN, int KS, int NC>
+__global__ __launch_bounds__((64 * kWaves<KS * kDeep<T> / 16, NC>)) void lora_up(const LoraArgs a, int ranks) {
+  constexpr int kW = kWaves<KS * kDeep<T> / 16, NC>, kThreads = 64 * kW, kRows = 16 * NC, kDepth = KS * kDeep<T>, kRow = kDepth + kRun<T>;
   // h as the matrix instruction takes it: the number itself (fp32), or its high part and the remainder
   constexpr int kPieces = sizeof(T) == 2 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) T hs[kPieces][kRows][kRow];
@@ -202,12 +206,11 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
   const int64_t row0 = int64_t(blockIdx.x) * kRows;
   Groups groups(a, row0, kRows, lane);
   const uint64_t valid = groups.rest;
-  const int over = share(groups.count()), parts = kWaves / over;
+  const int over = share(groups.count(), kW), parts = kW / over;
 
   // h of all rows: the splits' sums, in their order, times the adapter's scale; 16 lanes a row
-#pragma unroll
-  for (int p = 0; p < NC; ++p) {
-    const int row = p * 16 + int(threadIdx.x >> 4), l = threadIdx.x & 15;
+  for (int row = threadIdx.x >> 4; row < kRows; row += kThreads / 16) {
+    const int l = threadIdx.x & 15;
     const bool is = valid >> row & 1;
     const int id = __shfl(groups.id, row);
     const float scale = is ? (a.scales ? a.scales[id] : 1.f) : 0.f;
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
         const int m = col0 + (n16 >> 2) * 16 + n * 4 + (n16 & 3);
         const T* const Bm = B + int64_t(min(m, a.outer - 1)) * a.rank;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) bf[n][k] = load_frag<T, VEC>(Bm, k * kDeep<T> + g4 * kRun<T>, a.rank);
+        for (int k = 0; k < KS; ++k) bf[n][k] = load_frag<T, EVEN>(Bm, k * kDeep<T> + g4 * kRun<T>, a.rank);
       }
       const int col = col0 + g4 * 16, cols = min(16, a.outer - col);
 #pragma unroll
@@ -290,7 +293,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = 0.f;
         if (is) {
-          if (a.vector && cols == 16) {
+          if (cols == 16) {
             load_run<16>(y, v);
           } else {
 #pragma unroll
@@ -316,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
           const float f = std::is_same_v<T, f16> ? back[at] : 1.f;
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[j] += acc[j >> 2][j & 3] * f;
-          if (a.vector && cols == 16) {
+          if (cols == 16) {
             store_run<16>(out, v);
           } else {
 #pragma unroll
@@ -334,14 +337,10 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
     if (valid >> row & 1) continue;
     const T* const y = static_cast<const T*>(a.y) + (row0 + row) * a.y_row + col0;
     T* const out = static_cast<T*>(a.out) + (row0 + row) * a.out_row + col0;
-    if (a.vector) {
-      for (int i = threadIdx.x * kRun<T>; i < cols; i += kThreads * kRun<T>) {
-        if (i + kRun<T> <= cols) *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(y + i);
-        else
-          for (int j = i; j < cols; ++j) out[j] = y[j];
-      }
-    } else {
-      for (int i = threadIdx.x; i < cols; i += kThreads) out[i] = y[i];
+    for (int i = threadIdx.x * kRun<T>; i < cols; i += kThreads * kRun<T>) {
+      if (i + kRun<T> <= cols) store_any(out + i, load_any<frag<T>>(y + i));
+      else
+        for (int j = i; j < cols; ++j) out[j] = y[j];
     }
   }
 }
@@ -353,18 +352,17 @@ int row_tiles(int64_t rows) { return rows <= 1024 ? 1 : 4; }
 
 template <class T, int NR, int NC> void down(const LoraArgs& a, hipStream_t s) {
   const dim3 grid(unsigned((a.rows + 16 * NC - 1) / (16 * NC)), unsigned(a.splits));
-  const size_t lds = size_t(kWaves) * 16 * NC * (16 * NR + 4) * sizeof(float);
-  const bool vec = a.inner % kRun<T> == 0 && a.x_row % kRun<T> == 0 &&
-                   (reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.A)) % 16 == 0;
-  if (vec) launch_kernel(lora_down<T, true, NR, NC>, grid, kThreads, lds, s, a);
+  constexpr int kThreads = 64 * kWaves<NR, NC>;
+  const size_t lds = size_t(kWaves<NR, NC>) * 16 * NC * (16 * NR + 4) * sizeof(float);
+  if (a.inner % kRun<T> == 0) launch_kernel(lora_down<T, true, NR, NC>, grid, kThreads, lds, s, a);
   else launch_kernel(lora_down<T, false, NR, NC>, grid, kThreads, lds, s, a);
 }
 template <class T, int KS, int NC> void up(const LoraArgs& a, hipStream_t s) {
   const unsigned tiles = unsigned((a.outer + 63) / 64);
   const dim3 grid(unsigned((a.rows + 16 * NC - 1) / (16 * NC)), (tiles + unsigned(a.col_tiles) - 1) / unsigned(a.col_tiles));
-  const bool vec = a.rank % kRun<T> == 0 && reinterpret_cast<uintptr_t>(a.B) % 16 == 0;
   const int ranks = 16 * rank_tiles(a.rank);
-  if (vec) launch_kernel(lora_up<T, true, KS, NC>, grid, kThreads, 0, s, a, ranks);
+  constexpr int kThreads = 64 * kWaves<KS * kDeep<T> / 16, NC>;
+  if (a.rank % kRun<T> == 0) launch_kernel(lora_up<T, true, KS, NC>, grid, kThreads, 0, s, a, ranks);
   else launch_kernel(lora_up<T, false, KS, NC>, grid, kThreads, 0, s, a, ranks);
 }
 
@@ -407,12 +405,12 @@ void lora_add(LoraArgs a, hipStream_t s) {
     throw std::invalid_argument("lora_add: sizes");
   if (a.rows <= 0) return;
   if (a.rows > int64_t(1) << 31) throw std::invalid_argument("lora_add: too many rows for one call");
-  const int run = a.type == kF32 ? 4 : 8;
-  a.vector = a.y_row % run == 0 && a.out_row % run == 0 &&
-             (reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
   a.splits = splits_of(a.rows, a.inner);
-  // columns of a workgroup of "up", in tiles of 64: more of them where rows fill the chip, since each adds up h again
-  a.col_tiles = a.rows > 1024 ? 16 : 4;
+  // Columns of a workgroup of "up", in tiles of 64: as few as give the chip about two workgroups a CU, since a mixed
+  // batch's groups take them one after the other; more of a prompt, since each workgroup adds up h again.
+  const int64_t blocks = (a.rows + 16 * row_tiles(a.rows) - 1) / (16 * row_tiles(a.rows)), tiles = (a.outer + 63) / 64;
+  const int64_t each = blocks * tiles / 512;
+  a.col_tiles = int(each < 1 ? 1 : each > 16 ? 16 : each);
   switch (a.type) {
     case kF32: return dispatch<float>(a, s);
     case kF16: return dispatch<f16>(a, s);

@@ -88,6 +88,10 @@ template <class T, class C> __device__ __forceinline__ vec8<T> widen(uint32_t lo
   return r;
 }
 
+// Workgroups that a CU holds at once: what the registers of a kernel are limited to, and what the grid counts on.
+constexpr int resident(int padded_dim) { return padded_dim <= 64 ? 3 : padded_dim <= 128 ? 2 : 1; }
+constexpr int kCus = 256;
+
 struct Span {
   int lo, n, steps;  // first token that is seen, how many, steps of kStep (at least one)
 };
@@ -100,14 +104,14 @@ __device__ __forceinline__ Span span_of(const PagedAttentionArgs& a, int b) {
 }
 
 // Sum over the workgroup's threads of two numbers.
-template <int NT> __device__ __forceinline__ uint2 block_sum(uint2 v, uint2* lds) {
+__device__ __forceinline__ uint2 block_sum(uint2 v, uint2* lds) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v.x += __shfl_xor(v.x, o), v.y += __shfl_xor(v.y, o);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   uint2 s = make_uint2(0, 0);
 #pragma unroll
-  for (int i = 0; i < NT / 64; ++i) s.x += lds[i].x, s.y += lds[i].y;
+  for (int i = 0; i < kWaves; ++i) s.x += lds[i].x, s.y += lds[i].y;
   __syncthreads();
   return s;
 }
@@ -127,7 +131,7 @@ template <class T, class C, int DP> struct Shape {
 };
 
 template <class T, class C, int DP>
-__global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAttentionArgs a) {
+__global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel(const PagedAttentionArgs a) {
   using S = Shape<T, C, DP>;
   using V = typename S::V;
   __shared__ __attribute__((aligned(16))) char smem[kWaves * S::kWaveLds];
@@ -139,15 +143,19 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAt
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
   const int units = a.kv_heads * a.row_blocks;
 
-  // ---- this workgroup's run of steps
-  uint32_t mine = 0;
-  for (int b = threadIdx.x; b < a.batch; b += kThreads) mine += uint32_t(span_of(a, b).steps);
-  const uint32_t total = block_sum<kThreads>(make_uint2(mine, 0), sums).x * uint32_t(units);
-  const uint32_t per = (total + gridDim.x - 1) / gridDim.x;
-  uint32_t s = blockIdx.x * per;
-  const uint32_t end = s + per < total ? s + per : total;
-  if (s >= end) return;
-  // the request that holds step s: the one whose first step is the last at or before it
+  // ---- this workgroup's run of steps, and the request that its first one is in
+  uint32_t total = 0, per = 0, s = 0, end = 0;
+  const auto take = [&](uint32_t all) {
+    total = all * uint32_t(units);
+    per = (total + gridDim.x - 1) / gridDim.x;
+    s = blockIdx.x * per;
+    end = s + per < total ? s + per : total;
+  };
+  if (a.batch > kThreads) {  // else the scan below has the total at once
+    uint32_t mine = 0;
+    for (int b = threadIdx.x; b < a.batch; b += kThreads) mine += uint32_t(span_of(a, b).steps);
+    take(block_sum(make_uint2(mine, 0), sums).x);
+  }
   uint32_t before = 0;  // steps (of one unit) of the requests in front
   for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
     const int b = b0 + int(threadIdx.x);
@@ -166,6 +174,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAt
       if (i < wave) base += sums[i].x;
       chunk += sums[i].x;
     }
+    if (a.batch <= kThreads) take(chunk);
+    if (s >= end) return;  // the whole workgroup
     const uint32_t first = base + sc - st;
     if (st && first * units <= s && s < (first + st) * units) found[0] = uint32_t(b), found[1] = first;
     __syncthreads();
@@ -197,12 +207,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAt
         // the same order of dimensions as K's pieces have
         const int d = S::kQ8 ? (i >> 1) * 64 + g4 * 16 + (i & 1) * 8 : i * 32 + g4 * 8;
         vec8<T> x = {};
-        if (n16 < rows && d < dim) {
-          if (a.q_vector) x = *reinterpret_cast<const vec8<T>*>(q + d);
-          else
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = q[d + j];
-        }
+        if (n16 < rows && d < dim) x = load_any<vec8<T>>(q + d);
         qf[i] = x;
       }
     }
@@ -455,46 +460,95 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(const PagedAt
 }
 
 // Joins the partials of one query head: the workgroups of the first launch that
-// the (request, key head) pair's steps fell into, in their order.
-template <class T, int DP> __global__ __launch_bounds__(DP) void paged_attention_join(const PagedAttentionArgs a, int grid) {
-  __shared__ uint2 sums[DP / 64];
+// the (request, key head) pair's steps fell into, in their order.  All weights are
+// formed side by side, then DP / 4 lanes add a partial each; one after the other
+// they took 33 us for 47 partials, a round trip to memory each.
+template <class T, int DP> __global__ __launch_bounds__(kThreads) void paged_attention_join(const PagedAttentionArgs a, int grid) {
+  __shared__ uint2 sums[kWaves];
+  __shared__ float weight[resident(DP) * kCus], wave_of[2][kWaves];
+  __shared__ __attribute__((aligned(16))) f32x4 rows[kThreads];
   const int b = blockIdx.x / a.q_heads, h = blockIdx.x - b * a.q_heads, units = a.kv_heads * a.row_blocks;
   const int head = h / a.group, in_group = h - head * a.group, row = in_group & 15;
   const uint32_t unit = uint32_t(head * a.row_blocks + (in_group >> 4));
   uint2 mine = make_uint2(0, 0);
-  for (int i = threadIdx.x; i < a.batch; i += DP) {
+  for (int i = threadIdx.x; i < a.batch; i += kThreads) {
     const uint32_t st = uint32_t(span_of(a, i).steps);
     mine.x += st;
     mine.y += i < b ? st : 0;
   }
-  const uint2 all = block_sum<DP>(mine, sums);
+  const uint32_t steps = uint32_t(span_of(a, b).steps);
+  const uint2 all = block_sum(mine, sums);
   const uint32_t total = all.x * uint32_t(units), per = (total + uint32_t(grid) - 1) / uint32_t(grid);
-  const uint32_t steps = uint32_t(span_of(a, b).steps), first = all.y * uint32_t(units) + unit * steps;
-  const uint32_t w0 = first / per, w1 = (first + steps - 1) / per;
-  if (w0 == w1) return;  // finished where it was computed
-  const auto slot_of = [&](uint32_t w) { return 2 * int64_t(w) + (w * per >= first ? 0 : 1); };
-  float top = -INFINITY;
-  for (uint32_t w = w0; w <= w1; ++w) top = fmaxf(top, a.partial_ml[(slot_of(w) * a.partial_rows + row) * 2]);
-  const float ref = top > -INFINITY ? top : 0.f;
-  float sum = 0.f, x = 0.f;
-  const int d = threadIdx.x;
-#pragma unroll 4
-  for (uint32_t w = w0; w <= w1; ++w) {
-    const int64_t at = slot_of(w) * a.partial_rows + row;
-    const float f = __builtin_amdgcn_exp2f(a.partial_ml[at * 2] - ref);
-    sum += a.partial_ml[at * 2 + 1] * f;
-    if (d < a.dim) x += a.partial_o[at * DP + d] * f;
+  const uint32_t first = all.y * uint32_t(units) + unit * steps;
+  const int w0 = int(first / per), n = int((first + steps - 1) / per) - w0 + 1;
+  if (n == 1) return;  // finished where it was computed
+  const auto at = [&](int i) {  // the row of partial i
+    const uint32_t w = uint32_t(w0 + i);
+    return (2 * int64_t(w) + (w * per >= first ? 0 : 1)) * a.partial_rows + row;
+  };
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  constexpr int kEach = (resident(DP) * kCus + kThreads - 1) / kThreads;
+  float m[kEach], l[kEach], top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = k * kThreads + int(threadIdx.x);
+    m[k] = -INFINITY, l[k] = 0.f;
+    if (i < n) {
+      const float2 x = *reinterpret_cast<const float2*>(a.partial_ml + at(i) * 2);
+      m[k] = x.x, l[k] = x.y;
+    }
+    top = fmaxf(top, m[k]);
   }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) wave_of[0][wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_of[0][w]);
+  const float ref = top > -INFINITY ? top : 0.f;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = k * kThreads + int(threadIdx.x);
+    if (i < n) {
+      const float f = __builtin_amdgcn_exp2f(m[k] - ref);
+      weight[i] = f;
+      sum += l[k] * f;
+    }
+  }
+  sum = group_sum(sum, 64);
+  if (lane == 0) wave_of[1][wave] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) sum += wave_of[1][w];
+  constexpr int kLanes = DP / 4, kSide = kThreads / kLanes;  // lanes of a partial, partials side by side
+  const int side = threadIdx.x / kLanes, d = (threadIdx.x - side * kLanes) * 4;
+  f32x4 x = {};
+  if (d < a.dim) {
+#pragma unroll 4
+    for (int i = side; i < n; i += kSide) x += weight[i] * *reinterpret_cast<const f32x4*>(a.partial_o + at(i) * DP + d);
+  }
+  rows[threadIdx.x] = x;
+  __syncthreads();
   const int64_t out_row = int64_t(b) * a.q_heads + h;
-  if (d < a.dim) static_cast<T*>(a.out)[out_row * a.dim + d] = T(sum != 0.f ? x / sum : 0.f);
-  if (a.lse && d == 0) a.lse[out_row] = sum > 0.f || sum != sum ? (top + log2f(sum)) / kLog2e : -INFINITY;
+  if (side == 0 && d < a.dim) {
+    for (int i = 1; i < kSide; ++i) x += rows[i * kLanes + threadIdx.x];
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    float y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = x[r] * inv;
+    store_run<4>(static_cast<T*>(a.out) + out_row * a.dim + d, y);
+  }
+  if (a.lse && threadIdx.x == 0)
+    a.lse[out_row] = sum > 0.f || sum != sum ? (top + log2f(sum)) / kLog2e : -INFINITY;
 }
 
 template <class T, class C, int DP> void launch(const PagedAttentionArgs& a, hipStream_t s) {
   launch_kernel(paged_attention_kernel<T, C, DP>, dim3(unsigned(a.grid)), kThreads, 0, s, a);
   // a request of one step at most is never split
   if ((a.window > 0 && a.window < a.max_tokens ? a.window : a.max_tokens) > kStep)
-    launch_kernel(paged_attention_join<T, DP>, dim3(unsigned(a.batch * a.q_heads)), DP, 0, s, a, a.grid);
+    launch_kernel(paged_attention_join<T, DP>, dim3(unsigned(a.batch * a.q_heads)), kThreads, 0, s, a, a.grid);
 }
 
 template <class T, class C> void by_dim(const PagedAttentionArgs& a, hipStream_t s) {
@@ -516,9 +570,8 @@ int grid_of(int batch, int kv_heads, int row_blocks, int dim, int64_t max_tokens
   const int64_t seen = window > 0 && window < max_tokens ? window : max_tokens;
   const int64_t steps = (seen + kStep - 1) / kStep, pairs = int64_t(batch) * kv_heads * row_blocks;
   if (pairs > 0x7fffffff / steps) throw std::invalid_argument("paged_attention: too large for one call");
-  // as many workgroups as the 256 CUs hold at once (3 each, by registers; 1 of the widest)
-  const int64_t resident = 256 * (dim <= 128 ? 3 : 1), most = steps * pairs;
-  return int(most < resident ? most : resident);
+  const int64_t held = kCus * resident(padded_dim(dim)), most = steps * pairs;
+  return int(most < held ? most : held);
 }
 
 int64_t workspace_of(int64_t grid, int rows, int dim) { return 2 * grid * rows * (padded_dim(dim) + 2); }

@@ -11,7 +11,7 @@
 //
 // The pass is bound by reading x and writing y.  A head belongs to a group of
 // lanes of one wave, each holding V pairs as two vectors of V (16 bytes each
-// where sizes and alignment allow), so norm and rotation need no LDS exchange.
+// where the sizes allow), so norm and rotation need no LDS exchange.
 // A workgroup takes `tb` whole tokens: it computes their cosines and sines once,
 // one pair for each thread, into LDS, where all heads read them.  Recomputed by
 // each head they would cost as much time as the memory (about 40 instructions a
@@ -29,7 +29,8 @@ namespace {
 constexpr int kThreads = 256;
 
 template <class T, int V, bool IL>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const QkNormRopeArgs a, int lanes, int tb) {
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const QkNormRopeArgs a, int lanes, int lanes_log2, int tb,
+                                                              FastDiv by_half, FastDiv by_heads) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int half = a.dim / 2, heads = a.heads[0] + a.heads[1];
   float* const w_lds = lds;                 // [2][first values | second values of the pairs]
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const QkNormRope
     w_lds[which * a.dim + half + p] = v;
   }
   for (int i = threadIdx.x; i < nt * half; i += kThreads) {
-    const int t = i / half, p = i - t * half;
+    const int t = int(by_half.div(uint32_t(i))), p = i - t * half;
     float c = 1.f, s = 0.f;
     if (p < a.n_freq) {
       const double f = a.inv_freq64 ? static_cast<const double*>(a.inv_freq)[p]
@@ -76,10 +77,10 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const QkNormRope
   __syncthreads();
 
   constexpr int NS = V == 1 ? 4 : V == 2 ? 2 : 1;  // runs of V pairs for each lane: dim <= 512
-  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, per = kThreads / lanes;
+  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> lanes_log2, per = kThreads >> lanes_log2;
   // the lanes of a group share their slot, so a group is in the loop or out of it as a whole
   for (int it = slot; it < nt * heads; it += per) {
-    const int t = it / heads;
+    const int t = int(by_heads.div(uint32_t(it)));
     int h = it - t * heads;
     const int which = h >= a.heads[0];
     h -= which ? a.heads[0] : 0;
@@ -138,28 +139,24 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const QkNormRope
 
 template <class T, int V> void launch(const QkNormRopeArgs& a, hipStream_t s) {
   const int half = a.dim / 2;
-  int lanes = 1;
-  while (lanes < 64 && lanes * V < half) lanes *= 2;
+  int lanes = 1, log2 = 0;
+  while (lanes < 64 && lanes * V < half) lanes *= 2, ++log2;
   // whole tokens for each workgroup: one while they are few, so that each has a CU of its own
   int64_t tb = a.tokens / 1024;
   tb = tb < 1 ? 1 : tb > 4 ? 4 : tb;
   const unsigned grid = unsigned((a.tokens + tb - 1) / tb);
+  const FastDiv by_half{uint32_t(half)}, by_heads{uint32_t(a.heads[0] + a.heads[1])};
   const size_t lds = size_t(2 * a.dim + tb * a.dim) * sizeof(float);
-  if (a.interleaved) launch_kernel(qk_norm_rope_kernel<T, V, true>, grid, kThreads, lds, s, a, lanes, int(tb));
-  else launch_kernel(qk_norm_rope_kernel<T, V, false>, grid, kThreads, lds, s, a, lanes, int(tb));
+  if (a.interleaved) launch_kernel(qk_norm_rope_kernel<T, V, true>, grid, kThreads, lds, s, a, lanes, log2, int(tb), by_half,
+                                  by_heads);
+  else launch_kernel(qk_norm_rope_kernel<T, V, false>, grid, kThreads, lds, s, a, lanes, log2, int(tb), by_half,
+                                  by_heads);
 }
 
 template <class T> void dispatch(const QkNormRopeArgs& a, hipStream_t s) {
-  // the widest run that the split of the head, every row's start and the pointers allow
-  const int half = a.dim / 2;
-  int64_t all = half;
-  if (!a.interleaved) all |= a.n_freq | (half - a.n_freq);
-  int64_t bytes = 0;
-  for (int i = 0; i < 2; ++i) {
-    all |= a.x_token[i] | a.x_head[i] | a.out_token[i] | a.out_head[i];
-    bytes |= int64_t(reinterpret_cast<uintptr_t>(a.x[i]) | reinterpret_cast<uintptr_t>(a.out[i]));
-  }
-  const auto fits = [&](int v) { return all % v == 0 && bytes % (v * int(sizeof(T))) == 0; };
+  // the widest run that the head, and its turning and other parts, are made of
+  const int half = a.dim / 2, all = a.interleaved ? half : half | a.n_freq | (half - a.n_freq);
+  const auto fits = [&](int v) { return all % v == 0; };
   if constexpr (sizeof(T) == 2) {
     if (fits(8)) return launch<T, 8>(a, s);
   }

@@ -69,7 +69,8 @@ struct KvCacheArgs {
   FastDiv page;                  // slots of a page
   int64_t slots_total = 0;       // pages * page size
   int64_t rows = 0;
-  int heads = 0, dim = 0;        // dim <= 512
+  FastDiv heads;
+  int dim = 0;                   // <= 512
 };
 void kv_cache_write(const KvCacheArgs& a, hipStream_t stream);
 void kv_cache_read(const KvCacheArgs& a, hipStream_t stream);
@@ -80,7 +81,6 @@ void kv_cache_read(const KvCacheArgs& a, hipStream_t stream);
 struct PagedAttentionArgs {
   const void* q = nullptr;      // [batch, kv_heads * group, dim]
   int64_t q_batch = 0, q_head = 0;
-  int q_vector = 0;             // its rows start at multiples of 16 bytes
   int type = kBF16;             // of q and out: kF16 or kBF16
   const void* cache[2] = {};    // k, v: [pages, page size, kv_heads, dim], of `type` or 8 bits
   int64_t c_page[2] = {}, c_slot[2] = {}, c_head[2] = {};
@@ -125,7 +125,7 @@ struct LoraArgs {
   int type = kBF16;             // of all but ids and scales: kF32, kF16 or kBF16
   float* h = nullptr;           // workspace of lora_workspace() floats
   // filled in by lora_add()
-  int splits = 1, col_tiles = 1, vector = 0;
+  int splits = 1, col_tiles = 1;
 };
 int64_t lora_workspace(int64_t rows, int inner, int rank);
 void lora_add(LoraArgs a, hipStream_t stream);
