@@ -100,6 +100,13 @@ template <int V, class T> __device__ __forceinline__ void store_run(T* p, const 
   }
 }
 
+// The number of this thread's wave in its workgroup, and a value that all lanes of a
+// wave share, as scalars.  Matrix instructions run whatever the execution mask is, so
+// every condition around one has to be a scalar branch: under a mask that is empty
+// they would still add.
+__device__ __forceinline__ int wave_scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int wave_number() { return wave_scalar(int(threadIdx.x >> 6)); }
+
 // Sum / largest over the `width` (a power of two) neighbouring lanes of a group.
 __device__ __forceinline__ float group_sum(float v, int width) {
   for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);

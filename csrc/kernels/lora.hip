@@ -31,9 +31,10 @@
 namespace sca::kern {
 namespace {
 
-// Waves of a workgroup of NC row tiles: one for each group of a mixed batch's 16
-// rows (8 where the registers of a high rank allow no more), four for a prompt's.
-template <int NR, int NC> constexpr int kWaves = NC > 1 ? 4 : NR <= 2 ? 16 : 8;
+constexpr int kWaves = 4, kThreads = 64 * kWaves;  // of "up"; "down" has kDownWaves
+// A prompt's rows take eight waves over the inner dimension: 32 rows of 8192 fill the chip without splitting it over
+// workgroups, so h is written once instead of once a split.
+template <int ROWS> constexpr int kDownWaves = ROWS == 4 ? 4 : 8;
 
 using f32x4 = float __attribute__((ext_vector_type(4)));
 template <class T> constexpr int kRun = 16 / int(sizeof(T));   // elements of a lane's 16 bytes
@@ -53,12 +54,13 @@ __device__ __forceinline__ f32x4 mma(frag<float> a, frag<float> b, f32x4 c) {
   return c;
 }
 
-// kRun elements from p[at], zeros from `end` on.  EVEN: `end` is a multiple of kRun.
-template <class T, bool EVEN> __device__ __forceinline__ frag<T> load_frag(const T* p, int at, int end) {
+// kRun elements from p[at], zeros from `end` on.  Such a load hangs on a branch, and the compiler lets no later load
+// pass one: the loops below take full runs without it and leave the edges to a turn of their own.
+template <class T> __device__ __forceinline__ frag<T> load_edge(const T* p, int at, int end) {
   frag<T> x = {};
-  if (at + (EVEN ? 0 : kRun<T> - 1) < end) {
+  if (at + kRun<T> <= end) {
     x = load_any<frag<T>>(p + at);
-  } else if (!EVEN && at < end) {
+  } else if (at < end) {
 #pragma unroll
     for (int j = 0; j < kRun<T> - 1; ++j)
       if (at + j < end) x[j] = p[at + j];
@@ -66,33 +68,36 @@ template <class T, bool EVEN> __device__ __forceinline__ frag<T> load_frag(const
   return x;
 }
 
-// The rows of a workgroup by adapter.  Every wave walks them alike.
+// The rows of a workgroup by adapter; every wave has them alike.  A lane holds its
+// row's adapter and the set of rows that share it, found bit by bit of the adapter's
+// number: walking the groups one after the other, a ballot each, took longer than the
+// products of a mixed batch (16 groups: 4 us of 8).
 struct Groups {
-  uint64_t rest;
-  int id;  // of this lane's row
+  int id;          // of this lane's row, -1: none
+  uint64_t peers;  // rows of the same adapter
+  uint64_t rest;   // the first row of each group that is still to come
   __device__ Groups(const LoraArgs& a, int64_t row0, int rows, int lane) {
     int64_t v = -1;
     if (lane < rows && row0 + lane < a.rows) v = load_index(a.ids, a.ids64, row0 + lane);
     id = v >= 0 && v < a.adapters ? int(v) : -1;
-    rest = __ballot(id >= 0);
-  }
-  __device__ int count() const {
-    uint64_t r = rest;
-    int n = 0;
-    while (r) {
-      r &= ~__ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctzll(r)));
-      ++n;
+    peers = __ballot(id >= 0);
+    for (int bit = 0; (a.adapters - 1) >> bit; ++bit) {
+      const bool mine = id >> bit & 1;
+      const uint64_t set = __ballot(mine);
+      peers &= mine ? set : ~set;
     }
-    return n;
+    rest = __ballot(id >= 0 && __builtin_ctzll(peers) == lane);
   }
+  __device__ int count() const { return __popcll(rest); }
   // the next adapter and its rows
-  __device__ bool next(int& adapter, uint64_t& mask) {
-    if (!rest) return false;
-    adapter = __builtin_amdgcn_readlane(id, __builtin_ctzll(rest));
-    mask = __ballot(id == adapter);
-    rest &= ~mask;
-    return true;
+  __device__ void next(int& adapter, uint64_t& mask) {
+    const int first = __builtin_ctzll(rest);
+    rest &= rest - 1;
+    adapter = __builtin_amdgcn_readlane(id, first);
+    mask = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(peers >> 32), first))) << 32 |
+           uint32_t(__builtin_amdgcn_readlane(int(peers), first));
   }
+  __device__ void skip() { rest &= rest - 1; }
 };
 
 // Lane i of the result is the place of the i-th set bit of mask (anything behind the last).
@@ -104,149 +109,317 @@ __device__ __forceinline__ int set_bits(uint64_t mask, int lane) {
   return __builtin_amdgcn_ds_permute((mine ? rank : behind) * 4, lane);
 }
 
-// How `waves` (a power of two) share n groups: over as many of them as there are groups, up to the next power of two.
+// How 4 or 8 waves share n groups: over 1, 2, 4 or 8 of them.  The logarithm of that.
 __device__ __forceinline__ int share(int n, int waves) {
-  int over = 1;
-  while (over < n && over < waves) over *= 2;
-  return over;
+  const int log2 = n > 4 ? 3 : n > 2 ? 2 : n > 1 ? 1 : 0;
+  return waves == 4 && log2 == 3 ? 2 : log2;
+}
+
+// Workgroups go round the eight dies; each die takes neighbouring rows, whose adapters its L2 then holds once.
+__device__ __forceinline__ uint32_t row_block() {
+  const uint32_t n = gridDim.x, die = blockIdx.x & 7;
+  return die * (n >> 3) + min(die, n & 7) + (blockIdx.x >> 3);
 }
 
 // ---- h[split][row][rank] = sum over the split's part of the inner dimension
-// NR: rank tiles of 16, NC: row tiles of 16.
-template <class T, bool EVEN, int NR, int NC>
-__global__ __launch_bounds__((64 * kWaves<NR, NC>)) void lora_down(const LoraArgs a) {
-  extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][16 NC][16 NR + 4]
-  constexpr int kW = kWaves<NR, NC>, kThreads = 64 * kW, kRows = 16 * NC, kRow = 16 * NR + 4;
-  constexpr int kAhead = NR * NC >= 16 ? 2 : NR * NC >= 2 ? 4 : 8;  // steps whose loads are issued together
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
-  const int64_t row0 = int64_t(blockIdx.x) * kRows;
-  Groups groups(a, row0, kRows, lane);
-  const int over = share(groups.count(), kW), parts = kW / over;
-  const int my_part = wave / over;
-  // steps of kDeep: first those of the split, then those of this wave in it
-  const int steps = (a.inner + kDeep<T> - 1) / kDeep<T>;
+// NR: rank tiles of 16, ROWS: of a workgroup.
+template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWaves<ROWS>) void lora_down(const LoraArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float part[];  // [kW][ROWS][16 NR + 4]
+  constexpr int kW = kDownWaves<ROWS>, NC = (ROWS + 15) / 16, kRow = 16 * NR + 4;
+  constexpr int kAhead = NR == 1 && NC == 1 ? 8 : NR * NC >= 16 ? 2 : 4;  // steps whose loads are under way
+  const int wave = wave_number(), lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
+  const int64_t row0 = int64_t(row_block()) * ROWS;
+  Groups groups(a, row0, ROWS, lane);
+  const uint64_t valid = __ballot(groups.id >= 0);
+  const int over_log2 = share(groups.count(), kW), over = 1 << over_log2, parts = kW >> over_log2;
+  const int my_part = wave >> over_log2, my_turn = wave & (over - 1);
+  // steps of kDeep: first those of the split, then those of this wave in it; the last of all may be an edge
+  const int steps = (a.inner + kDeep<T> - 1) / kDeep<T>, full = a.inner / kDeep<T>;
   const int per = (steps + a.splits - 1) / a.splits, s0 = blockIdx.y * per, s1 = min(steps, s0 + per);
   const int wper = (per + parts - 1) / parts, w0 = min(s1, s0 + my_part * wper), w1 = min(s1, w0 + wper);
+  const int n = min(w1, full) - w0;
   float* const h = a.h + int64_t(blockIdx.y) * a.rows * (16 * NR);
 
   int adapter, turn = 0;
   uint64_t mask;
-  while (groups.next(adapter, mask)) {
-    if (turn++ % over != wave % over) continue;
-    const int place = set_bits(mask, lane), count = __popcll(mask), tiles = (count + 15) >> 4;
-    const T* const A = static_cast<const T*>(a.A) + int64_t(adapter) * a.rank * a.inner;
-    const T* xr[NC];
-    int at[NC];
+  // one group, in CT row tiles
+  const auto group = [&](auto tag) {
+    constexpr int CT = decltype(tag)::value;
+    const int place = set_bits(mask, lane), count = __popcll(mask);
+    const T* const A = static_cast<const T*>(a.A) + int64_t(adapter) * a.rank * a.inner + g4 * kRun<T>;
+    const T *xr[CT], *Ar[NR];
+    int at[CT];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
+    for (int c = 0; c < CT; ++c) {
       // a column behind the group's last row takes its first row again, and is not stored
       at[c] = __shfl(place, c * 16 + n16 < count ? c * 16 + n16 : 0);
-      xr[c] = static_cast<const T*>(a.x) + (row0 + at[c]) * a.x_row;
+      xr[c] = static_cast<const T*>(a.x) + (row0 + at[c]) * a.x_row + g4 * kRun<T>;
     }
-    const T* Ar[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) Ar[r] = A + int64_t(min(r * 16 + n16, a.rank - 1)) * a.inner;
-    f32x4 acc[NC][NR];
+    f32x4 acc[CT][NR];
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int r = 0; r < NR; ++r) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = w0; s < w1; s += kAhead) {
-      frag<T> xf[kAhead][NC], af[kAhead][NR];
+    frag<T> xf[kAhead][CT], af[kAhead][NR];
+    const auto issue = [&](int j, int i) {
+      const int k = (w0 + i) * kDeep<T>;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int k = (s + j) * kDeep<T> + g4 * kRun<T>, end = s + j < w1 ? a.inner : 0;
+      for (int r = 0; r < NR; ++r) af[j][r] = load_any<frag<T>>(Ar[r] + k);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) af[j][r] = load_frag<T, EVEN>(Ar[r], k, end);
+      for (int c = 0; c < CT; ++c) xf[j][c] = load_any<frag<T>>(xr[c] + k);
+    };
+    const auto multiply = [&](int j) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-          if (c < tiles) xf[j][c] = load_frag<T, EVEN>(xr[c], k, end);
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) acc[c][r] = mma(af[j][r], xf[j][c], acc[c][r]);
+    };
+    int s = 0;
+    if (n >= kAhead) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) issue(j, j);
+      for (; s + 2 * kAhead <= n; s += kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          multiply(j);
+          issue(j, s + j + kAhead);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
+      for (int j = 0; j < kAhead; ++j) multiply(j);
+      s += kAhead;
+    }
+    if (s < n) {  // fewer than kAhead are left
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-          if (c < tiles) {
+      for (int j = 0; j < kAhead - 1; ++j)
+        if (s + j < n) issue(j, s + j);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) acc[c][r] = mma(af[j][r], xf[j][c], acc[c][r]);
-          }
+      for (int j = 0; j < kAhead - 1; ++j)
+        if (s + j < n) multiply(j);
+    }
+    if (w0 <= full && full < w1) {
+      const int k = full * kDeep<T>, end = a.inner - g4 * kRun<T>;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) af[0][r] = load_edge<T>(Ar[r], k, end);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) xf[0][c] = load_edge<T>(xr[c], k, end);
+      multiply(0);
     }
     // lane: row n16 of the tile, ranks 16 r + 4 g4 + i
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < CT; ++c)
       if (c * 16 + n16 < count) {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          float* const to = parts == 1 ? h + (row0 + at[c]) * (16 * NR) : part + (my_part * kRows + at[c]) * kRow;
+          float* const to = parts == 1 ? h + (row0 + at[c]) * (16 * NR) : part + (my_part * ROWS + at[c]) * kRow;
           *reinterpret_cast<f32x4*>(to + r * 16 + g4 * 4) = acc[c][r];
         }
       }
+  };
+  while (groups.rest) {
+    if ((turn++ & (over - 1)) != my_turn) {
+      groups.skip();
+      continue;
+    }
+    groups.next(adapter, mask);
+    if (NC > 1 && __popcll(mask) > 16) group(std::integral_constant<int, NC>());
+    else group(std::integral_constant<int, 1>());
   }
   if (parts == 1) return;  // the same for the whole workgroup
   __syncthreads();
-  const uint64_t valid = __ballot(groups.id >= 0);
-  for (int i = threadIdx.x; i < kRows * NR * 4; i += kThreads) {
+  for (int i = threadIdx.x; i < ROWS * NR * 4; i += 64 * kW) {
     const int row = i / (NR * 4), r = (i - row * NR * 4) * 4;
     if (!(valid >> row & 1)) continue;
     f32x4 sum = *reinterpret_cast<const f32x4*>(part + row * kRow + r);
-    for (int p = 1; p < parts; ++p) sum += *reinterpret_cast<const f32x4*>(part + (p * kRows + row) * kRow + r);
+    for (int p = 1; p < parts; ++p) sum += *reinterpret_cast<const f32x4*>(part + (p * ROWS + row) * kRow + r);
     *reinterpret_cast<f32x4*>(h + (row0 + row) * (16 * NR) + r) = sum;
   }
 }
 
-// ---- out = y + B h.  KS: steps of the rank, NC: row tiles of 16.
-template <class T, bool EVEN, int KS, int NC>
-__global__ __launch_bounds__((64 * kWaves<KS * kDeep<T> / 16, NC>)) void lora_up(const LoraArgs a, int ranks) {
-  constexpr int kW = kWaves<KS * kDeep<T> / 16, NC>, kThreads = 64 * kW, kRows = 16 * NC, kDepth = KS * kDeep<T>, kRow = kDepth + kRun<T>;
+// ---- out = y + B h.  KS: steps of the rank.
+template <class T, bool EVEN, int KS, int ROWS>
+__global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks) {
+  constexpr int NC = (ROWS + 15) / 16, kDepth = KS * kDeep<T>, kRow = kDepth + kRun<T>;
   // h as the matrix instruction takes it: the number itself (fp32), or its high part and the remainder
   constexpr int kPieces = sizeof(T) == 2 ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) T hs[kPieces][kRows][kRow];
-  __shared__ float back[kRows];  // the power of two that fp16's h is over
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
-  const int64_t row0 = int64_t(blockIdx.x) * kRows;
-  Groups groups(a, row0, kRows, lane);
-  const uint64_t valid = groups.rest;
-  const int over = share(groups.count(), kW), parts = kW / over;
+  __shared__ __attribute__((aligned(16))) T hs[kPieces][ROWS][kRow];
+  __shared__ float back[ROWS];  // the power of two that fp16's h is over
+  const int wave = wave_number(), lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
+  const int64_t row0 = int64_t(row_block()) * ROWS;
 
-  // h of all rows: the splits' sums, in their order, times the adapter's scale; 16 lanes a row
-  for (int row = threadIdx.x >> 4; row < kRows; row += kThreads / 16) {
-    const int l = threadIdx.x & 15;
-    const bool is = valid >> row & 1;
-    const int id = __shfl(groups.id, row);
-    const float scale = is ? (a.scales ? a.scales[id] : 1.f) : 0.f;
-    f32x4 sum[(kDepth + 63) / 64];
-    float top = 0.f;
+  // h of a row is added up by 16 lanes, or by 64 that share the splits where rows are few.  Its loads go out before
+  // anything is known of the rows (what an unused row's h holds is dropped): a kernel of few rows is a chain of waits.
+  constexpr int kShare = ROWS == 4 ? 4 : 1, kPasses = ROWS * 16 * kShare / kThreads, kQuads = (kDepth + 63) / 64;
+  f32x4 sum[kPasses][kQuads];
+  const int l = threadIdx.x & 15, my_share = ROWS == 4 ? g4 : 0;
 #pragma unroll
-    for (int i = 0; i < (kDepth + 63) / 64; ++i) {
+  for (int p = 0; p < kPasses; ++p) {
+    const int64_t row = row0 + p * (kThreads / 16 / kShare) + int(threadIdx.x / (16 * kShare));
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
       const int r = (i * 16 + l) * 4;
-      sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (is && r < ranks) {
-        const float* const h = a.h + (row0 + row) * ranks + r;
+      sum[p][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (row < a.rows && r < ranks) {
+        const float* const h = a.h + row * ranks + r;
 #pragma unroll 4
-        for (int s = 0; s < a.splits; ++s) sum[i] += *reinterpret_cast<const f32x4*>(h + int64_t(s) * a.rows * ranks);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sum[i][j] = r + j < a.rank ? sum[i][j] * scale : 0.f;
-        top = fmaxf(top, fabsf(sum[i][j]));
+        for (int s = my_share; s < a.splits; s += kShare)
+          sum[p][i] += *reinterpret_cast<const f32x4*>(h + int64_t(s) * a.rows * ranks);
       }
     }
-    float over2 = 1.f;
+  }
+
+  Groups groups(a, row0, ROWS, lane);
+  const uint64_t valid = __ballot(groups.id >= 0);
+  const int over_log2 = share(groups.count(), kWaves), over = 1 << over_log2, parts = kWaves >> over_log2;
+  const int my_turn = wave & (over - 1);
+
+  // This wave's pieces of work are a group and 64 columns each; the next one's loads are under way while one is computed.
+  const int tile0 = blockIdx.y * a.col_tiles, tile1 = min(tile0 + a.col_tiles, (a.outer + 63) / 64);
+  // Of a piece's columns a lane has kPer runs of 16 bytes, and its row's four lanes lie side by side in each; so row i of
+  // product tile n is column 4 kRun (n / kPairs) + kRun (i / 4) + 4 (n % kPairs) + i % 4.
+  constexpr int kPer = 16 / kRun<T>, kPairs = kRun<T> / 4;
+  struct Piece {
+    int tile, count, at[NC];
+    frag<T> b[4][KS], y[NC][kPer];
+  };
+  const uint64_t all_groups = groups.rest;
+  int adapter = 0, turn = 0, place = 0, count = 0, tile = 0, lo = 0, hi = 0;  // tiles lo .. hi - 1 of this turn
+  const auto next = [&]() {
+    tile += parts;
+    if (tile < hi) return true;
+    if (lo + (wave >> over_log2) >= hi) return false;
+    while (groups.rest) {
+      if ((turn++ & (over - 1)) != my_turn) {
+        groups.skip();
+        continue;
+      }
+      uint64_t mask;
+      groups.next(adapter, mask);
+      place = set_bits(mask, lane), count = __popcll(mask);
+      tile = lo + (wave >> over_log2);
+      return true;
+    }
+    return false;
+  };
+  const auto load = [&](Piece& w, auto full) {
+    w.tile = tile, w.count = count;
+    const T* const B = static_cast<const T*>(a.B) + int64_t(adapter) * a.outer * a.rank;
+    const int col = tile * 64 + g4 * kRun<T>;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      // a column behind the group's last row takes its first row again, and is not stored
+      w.at[c] = __shfl(place, c * 16 + n16 < count ? c * 16 + n16 : 0);
+      const T* const y = static_cast<const T*>(a.y) + (row0 + w.at[c]) * a.y_row + col;
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        if constexpr (decltype(full)::value) w.y[c][q] = load_any<frag<T>>(y + q * 4 * kRun<T>);
+        else w.y[c][q] = load_edge<T>(y, q * 4 * kRun<T>, a.outer - col);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int m = tile * 64 + n / kPairs * 4 * kRun<T> + (n16 >> 2) * kRun<T> + n % kPairs * 4 + (n16 & 3);
+      const T* const Bm = B + int64_t(min(m, a.outer - 1)) * a.rank;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int r = k * kDeep<T> + g4 * kRun<T>;
+        if constexpr (EVEN) {
+          w.b[n][k] = load_any<frag<T>>(Bm + (r < a.rank ? r : 0));
+          if (r >= a.rank) w.b[n][k] = {};
+        } else {
+          w.b[n][k] = load_edge<T>(Bm, r, a.rank);
+        }
+      }
+    }
+  };
+  const auto compute = [&](const Piece& w, auto full) {
+    const int col = w.tile * 64 + g4 * kRun<T>;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (c * 16 >= w.count) break;
+      const int at = w.at[c];
+      f32x4 acc[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const frag<T> high = *reinterpret_cast<const frag<T>*>(&hs[0][at][k * kDeep<T> + g4 * kRun<T>]);
+        frag<T> low;
+        if constexpr (sizeof(T) == 2) low = *reinterpret_cast<const frag<T>*>(&hs[1][at][k * kDeep<T> + g4 * kRun<T>]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          acc[n] = mma(w.b[n][k], high, acc[n]);
+          if constexpr (sizeof(T) == 2) acc[n] = mma(w.b[n][k], low, acc[n]);
+        }
+      }
+      if (c * 16 + n16 < w.count) {
+        const float f = std::is_same_v<T, f16> ? back[at] : 1.f;
+        T* const out = static_cast<T*>(a.out) + (row0 + at) * a.out_row + col;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          float v[kRun<T>];
+#pragma unroll
+          for (int j = 0; j < kRun<T>; ++j) v[j] = float(w.y[c][q][j]) + acc[q * kPairs + j / 4][j % 4] * f;
+          const int left = a.outer - col - q * 4 * kRun<T>;
+          if (decltype(full)::value || left >= kRun<T>) {
+            store_run<kRun<T>>(out + q * 4 * kRun<T>, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kRun<T> - 1; ++j)
+              if (j < left) out[q * 4 * kRun<T> + j] = T(v[j]);
+          }
+        }
+      }
+    }
+  };
+
+  // The full tiles.  The first piece's loads go out before h is known.
+  const int tile_full = min(tile1, a.outer / 64);
+  lo = tile0, hi = tile_full, tile = hi;
+  bool more = next();
+  Piece now;
+  if (more) load(now, std::true_type());
+
+  // h to LDS: times the adapter's scale, in pieces
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int row = p * (kThreads / 16 / kShare) + int(threadIdx.x / (16 * kShare));
+    const int id = __shfl(groups.id, row);
+    const float scale = id >= 0 ? (a.scales ? a.scales[id] : 1.f) : 0.f;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int r = (i * 16 + l) * 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x = sum[p][i][j];
+        if constexpr (kShare == 4) {  // the splits in their order, by fours
+          x += __shfl_xor(x, 16);
+          x += __shfl_xor(x, 32);
+        }
+        x = id >= 0 && r + j < a.rank ? x * scale : 0.f;
+        sum[p][i][j] = x;
+        top = fmaxf(top, fabsf(x));
+      }
+    }
+    float over2 = 1.f, under = 1.f;
     if constexpr (std::is_same_v<T, f16>) {
       top = group_max(top, 16);
       const int e = int(__float_as_uint(top) >> 23);
       if (e > 1 && e < 254) {  // else zero, the least numbers, or not finite: as it is
         over2 = __uint_as_float(uint32_t(254 - e) << 23);
-        if (l == 0) back[row] = __uint_as_float(uint32_t(e) << 23);
-      } else if (l == 0) {
-        back[row] = 1.f;
+        under = __uint_as_float(uint32_t(e) << 23);
       }
     }
+    if (my_share) continue;
+    if (l == 0) back[row] = under;
 #pragma unroll
-    for (int i = 0; i < (kDepth + 63) / 64; ++i) {
+    for (int i = 0; i < kQuads; ++i) {
       const int r = (i * 16 + l) * 4;
       if (r < kDepth) {
-        f32x4 x = sum[i];
+        f32x4 x = sum[p][i];
         if constexpr (std::is_same_v<T, f16>) x *= over2;
         store_run<4>(&hs[0][row][r], reinterpret_cast<const float*>(&x));
         if constexpr (sizeof(T) == 2) {
@@ -263,77 +436,27 @@ __global__ __launch_bounds__((64 * kWaves<KS * kDeep<T> / 16, NC>)) void lora_up
   }
   __syncthreads();
 
-  const int tile0 = blockIdx.y * a.col_tiles, tile1 = min(tile0 + a.col_tiles, (a.outer + 63) / 64);
-  int adapter, turn = 0;
-  uint64_t mask;
-  while (groups.next(adapter, mask)) {
-    if (turn++ % over != wave % over) continue;
-    const int place = set_bits(mask, lane), count = __popcll(mask);
-    const T* const B = static_cast<const T*>(a.B) + int64_t(adapter) * a.outer * a.rank;
-    for (int tile = tile0 + wave / over; tile < tile1; tile += parts) {
-      const int col0 = tile * 64;
-      // row i of tile n is column 16 (i / 4) + 4 n + i % 4 of the 64: a lane's results are 16 neighbours
-      frag<T> bf[4][KS];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int m = col0 + (n16 >> 2) * 16 + n * 4 + (n16 & 3);
-        const T* const Bm = B + int64_t(min(m, a.outer - 1)) * a.rank;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) bf[n][k] = load_frag<T, EVEN>(Bm, k * kDeep<T> + g4 * kRun<T>, a.rank);
-      }
-      const int col = col0 + g4 * 16, cols = min(16, a.outer - col);
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (c * 16 >= count) break;
-        const bool is = c * 16 + n16 < count;
-        const int at = __shfl(place, is ? c * 16 + n16 : 0);
-        const T* const y = static_cast<const T*>(a.y) + (row0 + at) * a.y_row + col;
-        T* const out = static_cast<T*>(a.out) + (row0 + at) * a.out_row + col;
-        float v[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-        if (is) {
-          if (cols == 16) {
-            load_run<16>(y, v);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j < cols) v[j] = float(y[j]);
-          }
-        }
-        f32x4 acc[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const frag<T> hi = *reinterpret_cast<const frag<T>*>(&hs[0][at][k * kDeep<T> + g4 * kRun<T>]);
-          frag<T> lo;
-          if constexpr (sizeof(T) == 2) lo = *reinterpret_cast<const frag<T>*>(&hs[1][at][k * kDeep<T> + g4 * kRun<T>]);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            acc[n] = mma(bf[n][k], hi, acc[n]);
-            if constexpr (sizeof(T) == 2) acc[n] = mma(bf[n][k], lo, acc[n]);
-          }
-        }
-        if (is) {
-          const float f = std::is_same_v<T, f16> ? back[at] : 1.f;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] += acc[j >> 2][j & 3] * f;
-          if (cols == 16) {
-            store_run<16>(out, v);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j < cols) out[j] = T(v[j]);
-          }
-        }
-      }
+  if (more) {
+    while (next()) {
+      Piece then;
+      load(then, std::true_type());
+      compute(now, std::true_type());
+      now = then;
+    }
+    compute(now, std::true_type());
+  }
+  if (tile_full < tile1) {  // the last columns
+    groups.rest = all_groups, turn = 0;
+    lo = tile_full, hi = tile1, tile = hi;
+    while (next()) {
+      load(now, std::false_type());
+      compute(now, std::false_type());
     }
   }
   if (a.out == a.y) return;
   // rows without an adapter
   const int col0 = tile0 * 64, cols = min(a.outer, tile1 * 64) - col0;
-  for (int row = 0; row < kRows && row0 + row < a.rows; ++row) {
+  for (int row = 0; row < ROWS && row0 + row < a.rows; ++row) {
     if (valid >> row & 1) continue;
     const T* const y = static_cast<const T*>(a.y) + (row0 + row) * a.y_row + col0;
     T* const out = static_cast<T*>(a.out) + (row0 + row) * a.out_row + col0;
@@ -346,49 +469,48 @@ __global__ __launch_bounds__((64 * kWaves<KS * kDeep<T> / 16, NC>)) void lora_up
 }
 
 int rank_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
-// rows of a workgroup: 16 while rows are few, so that each adapter of a mixed batch has a wave of its own;
-// 64 of a prompt, which reads an adapter once for all of them
-int row_tiles(int64_t rows) { return rows <= 1024 ? 1 : 4; }
+// Few rows: 4 of a workgroup, so that each adapter of a mixed batch has a wave of its own (16 rows with 16 waves took
+// twice as long: one workgroup a CU, and all its waves wait for the same things).  Many: 32 or 64, which read an adapter
+// once for all of them.
+bool few(int64_t rows) { return rows <= 1024; }
 
-template <class T, int NR, int NC> void down(const LoraArgs& a, hipStream_t s) {
-  const dim3 grid(unsigned((a.rows + 16 * NC - 1) / (16 * NC)), unsigned(a.splits));
-  constexpr int kThreads = 64 * kWaves<NR, NC>;
-  const size_t lds = size_t(kWaves<NR, NC>) * 16 * NC * (16 * NR + 4) * sizeof(float);
-  if (a.inner % kRun<T> == 0) launch_kernel(lora_down<T, true, NR, NC>, grid, kThreads, lds, s, a);
-  else launch_kernel(lora_down<T, false, NR, NC>, grid, kThreads, lds, s, a);
+template <class T, int NR, int ROWS> void down(const LoraArgs& a, hipStream_t s) {
+  const dim3 grid(unsigned((a.rows + ROWS - 1) / ROWS), unsigned(a.splits));
+  constexpr int kW = kDownWaves<ROWS>;
+  const size_t lds = size_t(kW) * ROWS * (16 * NR + 4) * sizeof(float);
+  launch_kernel(lora_down<T, NR, ROWS>, grid, 64 * kW, lds, s, a);
 }
-template <class T, int KS, int NC> void up(const LoraArgs& a, hipStream_t s) {
+template <class T, int KS, int ROWS> void up(const LoraArgs& a, hipStream_t s) {
   const unsigned tiles = unsigned((a.outer + 63) / 64);
-  const dim3 grid(unsigned((a.rows + 16 * NC - 1) / (16 * NC)), (tiles + unsigned(a.col_tiles) - 1) / unsigned(a.col_tiles));
+  const dim3 grid(unsigned((a.rows + ROWS - 1) / ROWS), (tiles + unsigned(a.col_tiles) - 1) / unsigned(a.col_tiles));
   const int ranks = 16 * rank_tiles(a.rank);
-  constexpr int kThreads = 64 * kWaves<KS * kDeep<T> / 16, NC>;
-  if (a.rank % kRun<T> == 0) launch_kernel(lora_up<T, true, KS, NC>, grid, kThreads, 0, s, a, ranks);
-  else launch_kernel(lora_up<T, false, KS, NC>, grid, kThreads, 0, s, a, ranks);
+  if (a.rank % kRun<T> == 0) launch_kernel(lora_up<T, true, KS, ROWS>, grid, kThreads, 0, s, a, ranks);
+  else launch_kernel(lora_up<T, false, KS, ROWS>, grid, kThreads, 0, s, a, ranks);
 }
 
-template <class T, int NR, int NC> void both(const LoraArgs& a, hipStream_t s) {
-  down<T, NR, NC>(a, s);
-  up<T, (16 * NR + kDeep<T> - 1) / kDeep<T>, NC>(a, s);
+template <class T, int NR> void both(const LoraArgs& a, hipStream_t s) {
+  constexpr int KS = (16 * NR + kDeep<T> - 1) / kDeep<T>;
+  if (few(a.rows)) {
+    down<T, NR, 4>(a, s);
+    up<T, KS, 4>(a, s);
+  } else {
+    down<T, NR, 32>(a, s);
+    up<T, KS, 64>(a, s);
+  }
 }
 
 template <class T> void dispatch(const LoraArgs& a, hipStream_t s) {
-  const int nr = rank_tiles(a.rank);
-  if (row_tiles(a.rows) == 1) {
-    if (nr == 1) return both<T, 1, 1>(a, s);
-    if (nr == 2) return both<T, 2, 1>(a, s);
-    if (nr == 4) return both<T, 4, 1>(a, s);
-    return both<T, 8, 1>(a, s);
+  switch (rank_tiles(a.rank)) {
+    case 1: return both<T, 1>(a, s);
+    case 2: return both<T, 2>(a, s);
+    case 4: return both<T, 4>(a, s);
+    default: return both<T, 8>(a, s);
   }
-  if (nr == 1) return both<T, 1, 4>(a, s);
-  if (nr == 2) return both<T, 2, 4>(a, s);
-  if (nr == 4) return both<T, 4, 4>(a, s);
-  return both<T, 8, 4>(a, s);
 }
 
 int splits_of(int64_t rows, int inner) {
-  const int64_t blocks = (rows + 16 * row_tiles(rows) - 1) / (16 * row_tiles(rows));
-  // about two workgroups for each CU, of 256 of the inner dimension or more
-  const int64_t want = 512 / blocks, most = inner / 256;
+  // about two workgroups of four waves (one of eight) for each CU, of 256 (512) of the inner dimension or more
+  const int64_t want = few(rows) ? 2048 / rows : 8192 / rows, most = inner / (few(rows) ? 256 : 512);
   const int64_t n = want < most ? want : most;
   return int(n < 1 ? 1 : n);
 }
@@ -406,11 +528,11 @@ void lora_add(LoraArgs a, hipStream_t s) {
   if (a.rows <= 0) return;
   if (a.rows > int64_t(1) << 31) throw std::invalid_argument("lora_add: too many rows for one call");
   a.splits = splits_of(a.rows, a.inner);
-  // Columns of a workgroup of "up", in tiles of 64: as few as give the chip about two workgroups a CU, since a mixed
-  // batch's groups take them one after the other; more of a prompt, since each workgroup adds up h again.
-  const int64_t blocks = (a.rows + 16 * row_tiles(a.rows) - 1) / (16 * row_tiles(a.rows)), tiles = (a.outer + 63) / 64;
-  const int64_t each = blocks * tiles / 512;
-  a.col_tiles = int(each < 1 ? 1 : each > 16 ? 16 : each);
+  // Columns of a workgroup of "up", in tiles of 64: as few as give the chip four workgroups a CU (two of the larger),
+  // since a mixed batch's groups take them one after the other; at most 16.
+  const int64_t tiles = (a.outer + 63) / 64;
+  const int64_t each = few(a.rows) ? ((a.rows + 3) / 4 * tiles + 1023) / 1024 : ((a.rows + 63) / 64 * tiles + 511) / 512;
+  a.col_tiles = int(each > 16 ? 16 : each);
   switch (a.type) {
     case kF32: return dispatch<float>(a, s);
     case kF16: return dispatch<f16>(a, s);

@@ -140,13 +140,13 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
   __shared__ uint2 sums[kWaves];
   __shared__ uint32_t found[2];
 
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
+  const int wave = wave_number(), lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
   const int units = a.kv_heads * a.row_blocks;
 
   // ---- this workgroup's run of steps, and the request that its first one is in
   uint32_t total = 0, per = 0, s = 0, end = 0;
   const auto take = [&](uint32_t all) {
-    total = all * uint32_t(units);
+    total = uint32_t(wave_scalar(int(all))) * uint32_t(units);
     per = (total + gridDim.x - 1) / gridDim.x;
     s = blockIdx.x * per;
     end = s + per < total ? s + per : total;
@@ -182,8 +182,8 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
     before += chunk;
     if (before * units > s) break;
   }
-  int b = int(found[0]);
-  uint32_t first = found[1];
+  int b = wave_scalar(int(found[0]));
+  uint32_t first = uint32_t(wave_scalar(int(found[1])));
 
   const int dim = a.dim;
   const float to_log2 = a.scale * kLog2e;
@@ -486,7 +486,7 @@ template <class T, int DP> __global__ __launch_bounds__(kThreads) void paged_att
     const uint32_t w = uint32_t(w0 + i);
     return (2 * int64_t(w) + (w * per >= first ? 0 : 1)) * a.partial_rows + row;
   };
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = wave_number(), lane = threadIdx.x & 63;
   constexpr int kEach = (resident(DP) * kCus + kThreads - 1) / kThreads;
   float m[kEach], l[kEach], top = -INFINITY;
 #pragma unroll
