@@ -68,6 +68,28 @@ template <class T> __device__ __forceinline__ frag<T> load_edge(const T* p, int 
   return x;
 }
 
+// Memory and the matrix instruction want a wave's 16 rows in different lanes.  A load or store serves 16 neighbouring
+// lanes at a time, one cache access for each row among them, so memory has four lanes side by side on a row (lane =
+// 4 row + run); an operand has its rows side by side (lane = 16 run + row).  Loaded in the operand's order the cache's
+// accesses, four times as many, took two thirds of both kernels' time.  So loads are in memory's order, and the lanes
+// are exchanged in registers: to_operand() and, for the fp32 results, to_memory().
+__device__ __forceinline__ uint32_t from_lane(uint32_t x, int lane) {
+  return uint32_t(__builtin_amdgcn_ds_bpermute(lane * 4, int(x)));
+}
+template <class V> __device__ __forceinline__ V to_operand(const V& x, int lane) {
+  static_assert(sizeof(V) == 16, "a lane's run");
+  uint32_t w[4];
+  __builtin_memcpy(w, &x, 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = from_lane(w[i], (lane & 15) * 4 + (lane >> 4));
+  V y;
+  __builtin_memcpy(&y, w, 16);
+  return y;
+}
+__device__ __forceinline__ float to_memory(float x, int lane) {
+  return __uint_as_float(from_lane(__float_as_uint(x), (lane & 3) * 16 + (lane >> 2)));
+}
+
 // The rows of a workgroup by adapter; every wave has them alike.  A lane holds its
 // row's adapter and the set of rows that share it, found bit by bit of the adapter's
 // number: walking the groups one after the other, a ballot each, took longer than the
@@ -146,17 +168,17 @@ template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWave
   const auto group = [&](auto tag) {
     constexpr int CT = decltype(tag)::value;
     const int place = set_bits(mask, lane), count = __popcll(mask);
-    const T* const A = static_cast<const T*>(a.A) + int64_t(adapter) * a.rank * a.inner + g4 * kRun<T>;
+    const int row = lane >> 2, run = (lane & 3) * kRun<T>;  // in memory's order
+    const T* const A = static_cast<const T*>(a.A) + int64_t(adapter) * a.rank * a.inner + run;
     const T *xr[CT], *Ar[NR];
-    int at[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       // a column behind the group's last row takes its first row again, and is not stored
-      at[c] = __shfl(place, c * 16 + n16 < count ? c * 16 + n16 : 0);
-      xr[c] = static_cast<const T*>(a.x) + (row0 + at[c]) * a.x_row + g4 * kRun<T>;
+      const int at = __shfl(place, c * 16 + row < count ? c * 16 + row : 0);
+      xr[c] = static_cast<const T*>(a.x) + (row0 + at) * a.x_row + run;
     }
 #pragma unroll
-    for (int r = 0; r < NR; ++r) Ar[r] = A + int64_t(min(r * 16 + n16, a.rank - 1)) * a.inner;
+    for (int r = 0; r < NR; ++r) Ar[r] = A + int64_t(min(r * 16 + row, a.rank - 1)) * a.inner;
     f32x4 acc[CT][NR];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -171,10 +193,15 @@ template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWave
       for (int c = 0; c < CT; ++c) xf[j][c] = load_any<frag<T>>(xr[c] + k);
     };
     const auto multiply = [&](int j) {
+      frag<T> x[CT];
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
+      for (int c = 0; c < CT; ++c) x[c] = to_operand(xf[j][c], lane);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) acc[c][r] = mma(af[j][r], xf[j][c], acc[c][r]);
+      for (int r = 0; r < NR; ++r) {
+        const frag<T> A = to_operand(af[j][r], lane);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[c][r] = mma(A, x[c], acc[c][r]);
+      }
     };
     int s = 0;
     if (n >= kAhead) {
@@ -200,7 +227,7 @@ template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWave
         if (s + j < n) multiply(j);
     }
     if (w0 <= full && full < w1) {
-      const int k = full * kDeep<T>, end = a.inner - g4 * kRun<T>;
+      const int k = full * kDeep<T>, end = a.inner - run;
 #pragma unroll
       for (int r = 0; r < NR; ++r) af[0][r] = load_edge<T>(Ar[r], k, end);
 #pragma unroll
@@ -209,14 +236,16 @@ template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWave
     }
     // lane: row n16 of the tile, ranks 16 r + 4 g4 + i
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
+    for (int c = 0; c < CT; ++c) {
+      const int at = __shfl(place, c * 16 + n16 < count ? c * 16 + n16 : 0);
       if (c * 16 + n16 < count) {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          float* const to = parts == 1 ? h + (row0 + at[c]) * (16 * NR) : part + (my_part * ROWS + at[c]) * kRow;
+          float* const to = parts == 1 ? h + (row0 + at) * (16 * NR) : part + (my_part * ROWS + at) * kRow;
           *reinterpret_cast<f32x4*>(to + r * 16 + g4 * 4) = acc[c][r];
         }
       }
+    }
   };
   while (groups.rest) {
     if ((turn++ & (over - 1)) != my_turn) {
@@ -303,14 +332,16 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
     }
     return false;
   };
+  constexpr bool kExchange = ROWS > 4;
+  const int mem_row = kExchange ? lane >> 2 : n16, mem_run = (kExchange ? lane & 3 : g4) * kRun<T>;
   const auto load = [&](Piece& w, auto full) {
     w.tile = tile, w.count = count;
     const T* const B = static_cast<const T*>(a.B) + int64_t(adapter) * a.outer * a.rank;
-    const int col = tile * 64 + g4 * kRun<T>;
+    const int row = mem_row, run = mem_run, col = tile * 64 + run;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      // a column behind the group's last row takes its first row again, and is not stored
-      w.at[c] = __shfl(place, c * 16 + n16 < count ? c * 16 + n16 : 0);
+      // a row behind the group's last is its first again, and is not stored
+      w.at[c] = __shfl(place, c * 16 + row < count ? c * 16 + row : 0);
       const T* const y = static_cast<const T*>(a.y) + (row0 + w.at[c]) * a.y_row + col;
 #pragma unroll
       for (int q = 0; q < kPer; ++q) {
@@ -320,11 +351,11 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      const int m = tile * 64 + n / kPairs * 4 * kRun<T> + (n16 >> 2) * kRun<T> + n % kPairs * 4 + (n16 & 3);
+      const int m = tile * 64 + n / kPairs * 4 * kRun<T> + (row >> 2) * kRun<T> + n % kPairs * 4 + (row & 3);
       const T* const Bm = B + int64_t(min(m, a.outer - 1)) * a.rank;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const int r = k * kDeep<T> + g4 * kRun<T>;
+        const int r = k * kDeep<T> + run;
         if constexpr (EVEN) {
           w.b[n][k] = load_any<frag<T>>(Bm + (r < a.rank ? r : 0));
           if (r >= a.rank) w.b[n][k] = {};
@@ -335,11 +366,16 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
     }
   };
   const auto compute = [&](const Piece& w, auto full) {
-    const int col = w.tile * 64 + g4 * kRun<T>;
+    const int row = mem_row, col = w.tile * 64 + mem_run;
+    frag<T> b[4][KS];
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) b[n][k] = kExchange ? to_operand(w.b[n][k], lane) : w.b[n][k];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       if (c * 16 >= w.count) break;
-      const int at = w.at[c];
+      const int at = kExchange ? __shfl(w.at[c], n16 * 4) : w.at[c];  // the operand's row
       f32x4 acc[4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -350,25 +386,30 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
         if constexpr (sizeof(T) == 2) low = *reinterpret_cast<const frag<T>*>(&hs[1][at][k * kDeep<T> + g4 * kRun<T>]);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          acc[n] = mma(w.b[n][k], high, acc[n]);
-          if constexpr (sizeof(T) == 2) acc[n] = mma(w.b[n][k], low, acc[n]);
+          acc[n] = mma(b[n][k], high, acc[n]);
+          if constexpr (sizeof(T) == 2) acc[n] = mma(b[n][k], low, acc[n]);
         }
       }
-      if (c * 16 + n16 < w.count) {
-        const float f = std::is_same_v<T, f16> ? back[at] : 1.f;
-        T* const out = static_cast<T*>(a.out) + (row0 + at) * a.out_row + col;
+      const float f = std::is_same_v<T, f16> ? back[at] : 1.f;
+      float v[kPer][kRun<T>];
+#pragma unroll
+      for (int q = 0; q < kPer; ++q)
+#pragma unroll
+        for (int j = 0; j < kRun<T>; ++j) {
+          const float x = acc[q * kPairs + j / 4][j % 4] * f;
+          v[q][j] = float(w.y[c][q][j]) + (kExchange ? to_memory(x, lane) : x);
+        }
+      if (c * 16 + row < w.count) {
+        T* const out = static_cast<T*>(a.out) + (row0 + w.at[c]) * a.out_row + col;
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
-          float v[kRun<T>];
-#pragma unroll
-          for (int j = 0; j < kRun<T>; ++j) v[j] = float(w.y[c][q][j]) + acc[q * kPairs + j / 4][j % 4] * f;
           const int left = a.outer - col - q * 4 * kRun<T>;
           if (decltype(full)::value || left >= kRun<T>) {
-            store_run<kRun<T>>(out + q * 4 * kRun<T>, v);
+            store_run<kRun<T>>(out + q * 4 * kRun<T>, v[q]);
           } else {
 #pragma unroll
             for (int j = 0; j < kRun<T> - 1; ++j)
-              if (j < left) out[q * 4 * kRun<T> + j] = T(v[j]);
+              if (j < left) out[q * 4 * kRun<T> + j] = T(v[q][j]);
           }
         }
       }
@@ -438,10 +479,15 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
 
   if (more) {
     while (next()) {
-      Piece then;
-      load(then, std::true_type());
-      compute(now, std::true_type());
-      now = then;
+      if constexpr (KS > 4) {  // the registers hold one piece
+        compute(now, std::true_type());
+        load(now, std::true_type());
+      } else {
+        Piece then;
+        load(then, std::true_type());
+        compute(now, std::true_type());
+        now = then;
+      }
     }
     compute(now, std::true_type());
   }
