@@ -107,6 +107,13 @@ template <int V, class T> __device__ __forceinline__ void store_run(T* p, const 
 __device__ __forceinline__ int wave_scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int wave_number() { return wave_scalar(int(threadIdx.x >> 6)); }
 
+// Workgroups go round the eight dies, each with an L2 of its own.  This numbering of
+// the grid's x gives each die neighbouring numbers.
+__device__ __forceinline__ uint32_t die_order() {
+  const uint32_t n = gridDim.x, die = blockIdx.x & 7, more = n & 7;
+  return die * (n >> 3) + (die < more ? die : more) + (blockIdx.x >> 3);
+}
+
 // Sum / largest over the `width` (a power of two) neighbouring lanes of a group.
 __device__ __forceinline__ float group_sum(float v, int width) {
   for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);

@@ -137,12 +137,6 @@ __device__ __forceinline__ int share(int n, int waves) {
   return waves == 4 && log2 == 3 ? 2 : log2;
 }
 
-// Workgroups go round the eight dies; each die takes neighbouring rows, whose adapters its L2 then holds once.
-__device__ __forceinline__ uint32_t row_block() {
-  const uint32_t n = gridDim.x, die = blockIdx.x & 7;
-  return die * (n >> 3) + min(die, n & 7) + (blockIdx.x >> 3);
-}
-
 // ---- h[split][row][rank] = sum over the split's part of the inner dimension
 // NR: rank tiles of 16, ROWS: of a workgroup.
 template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWaves<ROWS>) void lora_down(const LoraArgs a) {
@@ -150,7 +144,7 @@ template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWave
   constexpr int kW = kDownWaves<ROWS>, NC = (ROWS + 15) / 16, kRow = 16 * NR + 4;
   constexpr int kAhead = NR == 1 && NC == 1 ? 8 : NR * NC >= 16 ? 2 : 4;  // steps whose loads are under way
   const int wave = wave_number(), lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
-  const int64_t row0 = int64_t(row_block()) * ROWS;
+  const int64_t row0 = int64_t(die_order()) * ROWS;  // a die's L2 then holds its rows' adapters once
   Groups groups(a, row0, ROWS, lane);
   const uint64_t valid = __ballot(groups.id >= 0);
   const int over_log2 = share(groups.count(), kW), over = 1 << over_log2, parts = kW >> over_log2;
@@ -276,7 +270,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
   __shared__ __attribute__((aligned(16))) T hs[kPieces][ROWS][kRow];
   __shared__ float back[ROWS];  // the power of two that fp16's h is over
   const int wave = wave_number(), lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
-  const int64_t row0 = int64_t(row_block()) * ROWS;
+  const int64_t row0 = int64_t(die_order()) * ROWS;
 
   // h of a row is added up by 16 lanes, or by 64 that share the splits where rows are few.  Its loads go out before
   // anything is known of the rows (what an unused row's h holds is dropped): a kernel of few rows is a chain of waits.

@@ -144,11 +144,13 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
   const int units = a.kv_heads * a.row_blocks;
 
   // ---- this workgroup's run of steps, and the request that its first one is in
+  // (a die's workgroups side by side: heads whose rows share cache lines meet in its L2)
+  const uint32_t group = die_order();
   uint32_t total = 0, per = 0, s = 0, end = 0;
   const auto take = [&](uint32_t all) {
     total = uint32_t(wave_scalar(int(all))) * uint32_t(units);
     per = (total + gridDim.x - 1) / gridDim.x;
-    s = blockIdx.x * per;
+    s = group * per;
     end = s + per < total ? s + per : total;
   };
   if (a.batch > kThreads) {  // else the scan below has the total at once
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
     __syncthreads();
     const bool whole = count == uint32_t(sp.steps);
     const int64_t out_row = int64_t(b) * a.q_heads + head * a.group + row0;
-    const int64_t slot = 2 * int64_t(blockIdx.x) + (step0 != 0 || s == blockIdx.x * per ? 0 : 1);
+    const int64_t slot = 2 * int64_t(group) + (step0 != 0 || s == group * per ? 0 : 1);
     if (threadIdx.x < uint32_t(rows)) {  // lanes of the first wave: n16 == threadIdx.x, so top and sum are this row's
       if (whole) {
         if (a.lse) a.lse[out_row + threadIdx.x] = sum > 0.f || sum != sum ? (top + log2f(sum)) / kLog2e : -INFINITY;
