@@ -217,9 +217,10 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
     // ---- the pipeline over this segment's tiles
     const int end_token = sp.lo + sp.n;
     const int32_t* const table = a.table + b * a.table_row;
-    const auto entry_of = [&](int t) -> int {  // the page of token t, or -1
-      return t < end_token ? table[a.page.div(uint32_t(t))] : -1;
-    };
+    // The page of token t; the last token's behind it.  Like every load of this loop it hangs on no branch: behind one the
+    // compiler waits for all loads before it, and the next tile's K went out a round trip to memory late.
+    const int last_token = max(end_token - 1, 0);
+    const auto entry_of = [&](int t) { return table[a.page.div(uint32_t(min(t, last_token)))]; };
     const C* const kc = static_cast<const C*>(a.cache[0]) + head * a.c_head[0];
     const C* const vc = static_cast<const C*>(a.cache[1]) + head * a.c_head[1];
     const float* const ks = a.cache_scale[0] + head * a.s_head[0];
@@ -276,8 +277,7 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
 #pragma unroll
     for (int h = 0; h < 2; ++h) entry[h] = entry_of(t + kStep + h * 16 + n16);
 
-    for (uint32_t it = 0; it < count; ++it, t += kStep) {
-      const bool more = it + 1 < count;
+    const auto tile = [&](auto more) {
       // scores of 32 tokens: lane has head n16, tokens 16 h + 4 g4 + r
       f32x4 sc[2];
 #pragma unroll
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
 #pragma unroll
           for (int r = 0; r < 4; ++r) sc[h][r] *= to_log2;
       }
-      if (more) {
+      if constexpr (decltype(more)::value) {
         int next[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) next[h] = entry_of(t + 2 * kStep + h * 16 + n16);
@@ -394,7 +394,9 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
         }
       }
       wave_sync();
-    }
+    };
+    for (uint32_t it = 1; it < count; ++it, t += kStep) tile(std::true_type());
+    tile(std::false_type());
 
     // ---- join the four waves
     l += __shfl_xor(l, 16);
