@@ -89,7 +89,10 @@ template <class T, class C> __device__ __forceinline__ vec8<T> widen(uint32_t lo
 }
 
 // Workgroups that a CU holds at once: what the registers of a kernel are limited to, and what the grid counts on.
-constexpr int resident(int padded_dim) { return padded_dim <= 64 ? 3 : padded_dim <= 128 ? 2 : 1; }
+constexpr int resident(int padded_dim, bool eight_bit) {
+  return padded_dim <= 64 ? 3 : padded_dim <= 128 ? (eight_bit ? 3 : 2) : eight_bit ? 2 : 1;
+}
+constexpr int kMostResident = 3;
 constexpr int kCus = 256;
 
 struct Span {
@@ -131,7 +134,7 @@ template <class T, class C, int DP> struct Shape {
 };
 
 template <class T, class C, int DP>
-__global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel(const PagedAttentionArgs a) {
+__global__ __launch_bounds__(kThreads, resident(DP, kQuantised<C>)) void paged_attention_kernel(const PagedAttentionArgs a) {
   using S = Shape<T, C, DP>;
   using V = typename S::V;
   __shared__ __attribute__((aligned(16))) char smem[kWaves * S::kWaveLds];
@@ -469,7 +472,7 @@ __global__ __launch_bounds__(kThreads, resident(DP)) void paged_attention_kernel
 // they took 33 us for 47 partials, a round trip to memory each.
 template <class T, int DP> __global__ __launch_bounds__(kThreads) void paged_attention_join(const PagedAttentionArgs a, int grid) {
   __shared__ uint2 sums[kWaves];
-  __shared__ float weight[resident(DP) * kCus], wave_of[2][kWaves];
+  __shared__ float weight[kMostResident * kCus], wave_of[2][kWaves];
   __shared__ __attribute__((aligned(16))) f32x4 rows[kThreads];
   const int b = blockIdx.x / a.q_heads, h = blockIdx.x - b * a.q_heads, units = a.kv_heads * a.row_blocks;
   const int head = h / a.group, in_group = h - head * a.group, row = in_group & 15;
@@ -491,7 +494,7 @@ template <class T, int DP> __global__ __launch_bounds__(kThreads) void paged_att
     return (2 * int64_t(w) + (w * per >= first ? 0 : 1)) * a.partial_rows + row;
   };
   const int wave = wave_number(), lane = threadIdx.x & 63;
-  constexpr int kEach = (resident(DP) * kCus + kThreads - 1) / kThreads;
+  constexpr int kEach = kMostResident * kCus / kThreads;
   float m[kEach], l[kEach], top = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
@@ -570,11 +573,11 @@ template <class T> void by_cache(const PagedAttentionArgs& a, hipStream_t s) {
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-int grid_of(int batch, int kv_heads, int row_blocks, int dim, int64_t max_tokens, int window) {
+int grid_of(int batch, int kv_heads, int row_blocks, int dim, bool eight_bit, int64_t max_tokens, int window) {
   const int64_t seen = window > 0 && window < max_tokens ? window : max_tokens;
   const int64_t steps = (seen + kStep - 1) / kStep, pairs = int64_t(batch) * kv_heads * row_blocks;
   if (pairs > 0x7fffffff / steps) throw std::invalid_argument("paged_attention: too large for one call");
-  const int64_t held = kCus * resident(padded_dim(dim)), most = steps * pairs;
+  const int64_t held = kCus * resident(padded_dim(dim), eight_bit), most = steps * pairs;
   return int(most < held ? most : held);
 }
 
@@ -599,12 +602,13 @@ int64_t paged_attention_plan(PagedAttentionArgs& a) {
   a.row_blocks = (a.group + 15) / 16;
   a.partial_rows = a.group < 16 ? a.group : 16;
   if (int64_t(a.batch) * a.q_heads > 0x7fffffff) throw std::invalid_argument("paged_attention: too large for one call");
-  a.grid = grid_of(a.batch, a.kv_heads, a.row_blocks, a.dim, a.max_tokens, a.window);
+  a.grid = grid_of(a.batch, a.kv_heads, a.row_blocks, a.dim, width == 1, a.max_tokens, a.window);
   return workspace_of(a.grid, a.partial_rows, a.dim);
 }
 
-int64_t paged_attention_workspace(int batch, int kv_heads, int group, int dim, int64_t max_tokens, int window) {
-  return workspace_of(grid_of(batch, kv_heads, (group + 15) / 16, dim, max_tokens, window), group < 16 ? group : 16, dim);
+int64_t paged_attention_workspace(int batch, int kv_heads, int group, int dim, bool eight_bit, int64_t max_tokens,
+                                  int window) {
+  return workspace_of(grid_of(batch, kv_heads, (group + 15) / 16, dim, eight_bit, max_tokens, window), group < 16 ? group : 16, dim);
 }
 
 void paged_attention(const PagedAttentionArgs& a, hipStream_t s) {

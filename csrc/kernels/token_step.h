@@ -107,7 +107,8 @@ struct PagedAttentionArgs {
 // partial_ml lies at its start, partial_o behind its 4 * grid * partial_rows floats.
 int64_t paged_attention_plan(PagedAttentionArgs& a);
 void paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
-int64_t paged_attention_workspace(int batch, int kv_heads, int group, int dim, int64_t max_tokens, int window);
+int64_t paged_attention_workspace(int batch, int kv_heads, int group, int dim, bool eight_bit, int64_t max_tokens,
+                                  int window);
 
 // out = y + scale[a] * (x A[a]^T) B[a]^T for each row's adapter a.
 struct LoraArgs {

@@ -164,17 +164,24 @@ class KVCache(NamedTuple):
 
 def kv_cache(pages: int, page_size: int, heads: int, dim: int, dtype=None, device="cuda") -> KVCache:
     """A zeroed cache.  ``dtype``: bf16 (the default), fp16 or fp32, or
-    float8_e4m3fn or int8 for one that is quantised as it is written."""
+    float8_e4m3fn or int8 for one that is quantised as it is written.
+
+    A page keeps the rows of a head together (the tensors are transposed views):
+    attention reads one head at a time, and where rows are not whole 128-byte
+    lines it would otherwise fetch its neighbours' too (36 requests of 3000
+    tokens, 12 heads: 47 against 68 us at e4m3 and dim 64, 129 against 139 at
+    bf16 and dim 128).
+    """
     dtype = dtype or torch.bfloat16
     if dtype not in _TYPE:
         raise TypeError(f"dtype must be one of {[str(d) for d in _TYPE]}, got {dtype}")
     if min(pages, page_size, heads, dim) < 1:
         raise ValueError("pages, page_size, heads and dim must be positive")
-    shape = (pages, page_size, heads, dim)
-    k, v = torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
+    shape = (pages, heads, page_size, dim)
+    k, v = (torch.zeros(shape, dtype=dtype, device=device).transpose(1, 2) for _ in range(2))
     if dtype in _FLOATS:
         return KVCache(k, v)
-    return KVCache(k, v, *(torch.ones(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+    return KVCache(k, v, *(torch.ones(shape[:3], dtype=torch.float32, device=device).transpose(1, 2) for _ in range(2)))
 
 
 def _cache(cache, device=None):
@@ -259,7 +266,7 @@ _workspace = None
 
 
 def _attention_workspace(*sizes):
-    """fp32 numbers of workspace for (batch, kv heads, group, dim, tokens, window)."""
+    """fp32 numbers of workspace for (batch, kv heads, group, dim, 8 bits, tokens, window)."""
     global _workspace
     if _workspace is None:
         _workspace = functools.lru_cache(maxsize=1024)(_k().paged_attention_workspace)
@@ -315,7 +322,7 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
             raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
     lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
     if B:
-        n = _attention_workspace(B, H, Hq // H, D, W * page, window)
+        n = _attention_workspace(B, H, Hq // H, D, c.dtype.itemsize == 1, W * page, window)
         ws = torch.empty(n, dtype=torch.float32, device=dev)
         _launch(q, _k().paged_attention, q.data_ptr(), q.stride(0), q.stride(1), _TYPE[q.dtype], ptrs, cst, _TYPE[c.dtype],
                 pages, page, page_table.data_ptr(), page_table.stride(0), W, lengths.data_ptr(), B, H, Hq // H, D, window,

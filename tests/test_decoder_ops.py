@@ -141,7 +141,7 @@ def test_kv_cache_write_and_read(T, pages, page, heads, dim, cache, dtype):
     assert ops.kv_cache_write(c, k.cuda(), v.cuda(), slots.cuda()) is c
     kept = slots >= 0
     for x, codes, scales in ((k, c.k, c.k_scales), (v, c.v, c.v_scales)):
-        flat = codes.cpu().view(-1, heads, dim)
+        flat = codes.cpu().reshape(-1, heads, dim)
         if scales is None:
             want = torch.zeros((pages * page, heads, dim), dtype=ct)
             want[slots[kept]] = x[kept].to(ct)
@@ -151,11 +151,11 @@ def test_kv_cache_write_and_read(T, pages, page, heads, dim, cache, dtype):
             want = torch.zeros((pages * page, heads, dim))
             ws = torch.ones((pages * page, heads))
             want[slots[kept]], ws[slots[kept]] = qc.float(), qs
-            assert torch.equal(flat.float(), want) and torch.equal(scales.cpu().view(-1, heads), ws)
+            assert torch.equal(flat.float(), want) and torch.equal(scales.cpu().reshape(-1, heads), ws)
             # e4m3: half a step of the value, 2^-4 of it, or where it is subnormal 2^-10 scales, with scale <= top / 224.
             # int8: |code - x / s| <= 1/2 + 127 * 2^-24 (the quotient's own rounding) < 1/2 (1 + 2^-16) and
             # s <= top / 127 (1 + 2^-24)^2, so |code * s - x| <= top / 254 (1 + 2^-15).
-            got = values(flat, scales.cpu().view(-1, heads))[slots[kept]]
+            got = values(flat, scales.cpu().reshape(-1, heads))[slots[kept]]
             top = x[kept].double().abs().amax(-1, keepdim=True)
             step = x[kept].double().abs() * 2.0 ** -4 + top * 2.0 ** -17 if ct == E4M3 else top / 254 * (1 + 2.0 ** -15)
             assert bool((got - x[kept].double()).abs().le(step).all())
@@ -166,9 +166,9 @@ def test_kv_cache_write_and_read(T, pages, page, heads, dim, cache, dtype):
         od = out or (ct if ct.itemsize > 1 else torch.bfloat16)
         assert kr.dtype == od
         for r, codes, scales in ((kr, c.k, c.k_scales), (vr, c.v, c.v_scales)):
-            flat = codes.cpu().view(-1, heads, dim).float()
+            flat = codes.cpu().reshape(-1, heads, dim).float()
             if scales is not None:
-                flat = flat * scales.cpu().view(-1, heads)[..., None]
+                flat = flat * scales.cpu().reshape(-1, heads)[..., None]
             ok = (ask >= 0) & (ask < pages * page)
             want = torch.where(ok[:, None, None], flat[torch.where(ok, ask, 0)], torch.zeros(())).to(od)
             assert torch.equal(r.cpu(), want)
@@ -190,7 +190,7 @@ def test_kv_cache_scales_over_the_whole_range(cache):
     ops.kv_cache_write(c, k.cuda(), k.cuda(), slots.cuda())
     codes, scales = ops.token_step.kv_quantise_ref(k, ct)
     n = len(k)
-    assert same(c.k_scales.cpu().view(-1, 1)[:n], scales) and same(c.v.cpu().view(-1, 1, 32)[:n].float(), codes.float())
+    assert same(c.k_scales.cpu().reshape(-1, 1)[:n], scales) and same(c.v.cpu().reshape(-1, 1, 32)[:n].float(), codes.float())
     kr, _ = ops.kv_cache_read(c, slots.cuda(), dtype=torch.float32)
     assert torch.isfinite(kr[:len(tops) - 1]).all() and kr[len(tops):].isnan().all()
 
@@ -459,3 +459,255 @@ def test_lora_add_large_and_infinite_values():
     e = ops.lora_add(torch.empty((0, M), device="cuda"), torch.empty((0, K), device="cuda"), A.float().cuda(), B.float().cuda(),
                      torch.empty(0, dtype=torch.int32, device="cuda"))
     assert e.shape == (0, M)
+
+
+# ----------------------------------------------------- together, as they are used
+class Step(torch.nn.Module):
+    """One decoder attention block over a cache that it keeps: projection with adapters, norm and rotation, cache, attention."""
+
+    def __init__(self, hidden, Hq, H, D, tenants, pages, page, cache, g):
+        super().__init__()
+        self.Hq, self.H, self.D, self.page = Hq, H, D, page
+        n = (Hq + 2 * H) * D
+        self.w = (randn(g, n, hidden) * hidden ** -0.5).bfloat16().cuda()
+        self.A, self.B = (randn(g, tenants, 8, hidden) * hidden ** -0.5).bfloat16().cuda(), (randn(g, tenants, n, 8) * 0.3).bfloat16().cuda()
+        self.qn, self.kn = ((1 + 0.1 * randn(g, D)).bfloat16().cuda() for _ in range(2))
+        self.inv = (10000.0 ** (-torch.arange(0, D, 2) / D)).cuda()
+        self.cache = ops.kv_cache(pages, page, H, D, dtype=cache)
+
+    def forward(self, x, tenant, positions, table):
+        Hq, H, D = self.Hq, self.H, self.D
+        y = x @ self.w.T
+        y = ops.lora_add(y, x, self.A, self.B, tenant, out=y).view(len(x), -1, D)
+        q, k = ops.qk_norm_rope(y[:, :Hq], y[:, Hq:Hq + H], self.qn, self.kn, positions, self.inv)
+        at = positions.clamp_min(0).long()  # padding has no place in the table
+        slots = table.long().gather(1, at[:, None] // self.page)[:, 0] * self.page + at % self.page
+        slots = torch.where(positions >= 0, slots, -1)
+        ops.kv_cache_write(self.cache, k, y[:, Hq + H:], slots)
+        return ops.paged_attention(q, self.cache, table, positions + 1)
+
+
+def step_inputs(g, T, tenants, table_width, page, at):
+    """Requests at position `at` + i, the last one padding."""
+    x = randn(g, T, 256, dtype=torch.bfloat16).cuda()
+    pos = (at + torch.arange(T) * 3).int()
+    pos[-1] = -1
+    return x, (torch.arange(T) % (tenants + 1) - 1).int().cuda(), pos.cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", [torch.bfloat16, E4M3, torch.int8])
+def test_steps_together_and_replayed(cache):
+    """Eight decode steps eagerly against 64 bits, then the same steps as replays of one captured graph: the same bits."""
+    T, page, W, Hq, H, D, tenants = 5, 16, 4, 8, 2, 64, 3
+    g = gen(21)
+    m = Step(256, Hq, H, D, tenants, T * W, page, cache, g)
+    table = torch.randperm(T * W, generator=g).int().view(T, W).cuda()
+    inputs = [step_inputs(g, T, tenants, W, page, 7 + i) for i in range(8)]
+    for i, (x, tenant, pos) in enumerate(inputs):  # the prompts' tokens: random rows at the positions before
+        if i == 0:
+            for t in range(T - 1):
+                n = int(pos[t])
+                s = table[t].long().cpu()[torch.arange(n) // page] * page + torch.arange(n) % page
+                ops.kv_cache_write(m.cache, *(randn(g, n, H, D, dtype=torch.bfloat16).cuda() for _ in range(2)), s.cuda())
+    start = [None if c is None else c.clone() for c in m.cache]
+    outs = []
+    with torch.no_grad():
+        for x, tenant, pos in inputs:
+            out = m(x, tenant, pos, table)
+            outs.append(out.clone())
+            # the last piece against 64 bits on the cache as it is
+            y = x @ m.w.T
+            ops.lora_add(y, x, m.A, m.B, tenant, out=y)
+            q, _ = ops.qk_norm_rope(y.view(T, -1, D)[:, :Hq], y.view(T, -1, D)[:, Hq:Hq + H], m.qn, m.kn, pos, m.inv)
+            c = ops.KVCache(*(None if t is None else t.cpu() for t in m.cache))
+            attention_check(out, None, q.cpu(), c, table.cpu(), pos.cpu() + 1)
+            assert not out[-1].any()
+    end = [None if c is None else c.clone() for c in m.cache]
+    # captured: static inputs, replayed with eager work in between
+    sx, st, sp = (t.clone() for t in inputs[0])
+    side = torch.cuda.Stream()
+    with torch.no_grad(), torch.cuda.stream(side):
+        m(sx, st, sp, table)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph, stream=side):
+        sy = m(sx, st, sp, table)
+    for c, b in zip(m.cache, start):
+        if c is not None:
+            c.copy_(b)
+    for (x, tenant, pos), want in zip(inputs, outs):
+        sx.copy_(x), st.copy_(tenant), sp.copy_(pos)
+        graph.replay()
+        junk = ops.lora_add(x @ m.w.T, x, m.A, m.B, tenant)  # eager work of the same shapes
+        torch.cuda.synchronize()
+        assert torch.equal(sy, want) and junk.shape[0] == T
+    for c, b in zip(m.cache, end):
+        assert c is None or torch.equal(c.float(), b.float())
+
+
+@pytest.mark.gpu
+def test_two_graphs_and_two_streams_share_nothing():
+    """Two captured calls replayed at once on two streams give what each gives alone."""
+    g = gen(33)
+    cases = []
+    for lens in ([3000, 17, 400], [1200, 2500, 1]):
+        q, c, table, lengths = attention_inputs(g, lens, 16, 4, 128, 16, torch.bfloat16, "same")
+        cases.append((q.cuda(), to_gpu(c), table.cuda(), lengths.cuda()))
+    want = [ops.paged_attention(*c) for c in cases]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in cases]
+    for c, s in zip(cases, streams):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            outs.append(ops.paged_attention(*c))
+        graphs.append(graph)
+    for _ in range(5):
+        for o in outs:
+            o.fill_(math.nan)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
+
+
+@pytest.mark.gpu
+def test_served_module_replays_adapters_through_graphs():
+    """A torch module of linear layers with an adapter beside each, served by GraphedModule."""
+    from seldon_core_amd.models.graphed import GraphedModule
+
+    class M(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a = torch.nn.Linear(64, 96)
+            self.A, self.B = torch.nn.Parameter(torch.randn(2, 8, 64) * 0.1), torch.nn.Parameter(torch.randn(2, 96, 8))
+
+        def forward(self, x):  # the last column says whose row it is
+            y = self.a(x[:, :-1])
+            return ops.lora_add(y, x[:, :-1], self.A, self.B, x[:, -1].to(torch.int32))
+
+    m = GraphedModule(M(), max_batch=16)
+    X = torch.randn(37, 65)
+    X[:, -1] = torch.arange(37) % 3 - 1
+    got = m(X.numpy())
+    assert m.graph_error is None and m.replays >= 3
+    mod = m.module.cpu()
+    x, ids = X[:, :-1], X[:, -1].int()
+    want, mag = ops.token_step.lora_add_ref((x.double() @ mod.a.weight.double().T + mod.a.bias.double()).detach(), x, mod.A.detach(),
+                                            mod.B.detach(), ids)
+    lin = x.abs().double() @ mod.a.weight.detach().abs().double().T + mod.a.bias.detach().abs().double()
+    close(torch.from_numpy(got), want, torch.float32, 200 * 2.0 ** -24 * (mag + lin))  # sums of 64 and 8 products, and y's own
+
+
+# ---------------------------------------------------------------- refusals
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+def test_refusals_before_anything_is_launched():
+    """On fake GPU tensors: every refusal comes from the host's checks."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    bf, f32, i32 = torch.bfloat16, torch.float32, torch.int32
+    with pytest.raises(ValueError, match="GPU tensor"):
+        ops.qk_norm_rope(torch.zeros(2, 2, 4), torch.zeros(2, 2, 4), None, None, torch.zeros(2), torch.zeros(2))
+    with pytest.raises(ValueError, match="GPU tensor"):
+        ops.lora_add(*[torch.zeros(2, 2)] * 5)
+    with FakeTensorMode():
+        def t(*shape, dtype=bf):
+            return torch.empty(shape, dtype=dtype, device="cuda")
+
+        q, k, pos, inv = t(4, 8, 64), t(4, 2, 64), t(4, dtype=i32), t(32, dtype=f32)
+
+        def refuse(error, match, fn, *a, **kw):
+            with pytest.raises(error, match=match):
+                fn(*a, **kw)
+
+        rope = ops.qk_norm_rope
+        refuse(TypeError, "k must be", rope, q, t(4, 2, 64, dtype=f32), None, None, pos, inv)
+        refuse(TypeError, "q must be", rope, t(4, 8, 64, dtype=torch.float64), k, None, None, pos, inv)
+        refuse(ValueError, "agree", rope, q, t(5, 2, 64), None, None, pos, inv)
+        refuse(ValueError, "even", rope, t(4, 8, 63), t(4, 2, 63), None, None, pos, inv)
+        refuse(ValueError, "even", rope, t(4, 8, 514), t(4, 2, 514), None, None, pos, inv)
+        refuse(ValueError, "last dimension", rope, t(4, 64, 8).transpose(1, 2), k, None, None, pos, inv)
+        refuse(ValueError, "q_weight must have", rope, q, k, t(63), None, pos, inv)
+        refuse(TypeError, "one type", rope, q, k, t(64), t(64, dtype=f32), pos, inv)
+        refuse(ValueError, "positions must have", rope, q, k, None, None, t(5, dtype=i32), inv)
+        refuse(TypeError, "positions", rope, q, k, None, None, t(4, dtype=f32), inv)
+        refuse(ValueError, "turns", rope, q, k, None, None, pos, t(33, dtype=f32))
+        refuse(ValueError, r"out\[0\]", rope, q, k, None, None, pos, inv, out=(t(4, 8, 32), k))
+        refuse(RuntimeError, "forward only", rope, q.clone().requires_grad_(), k, None, None, pos, inv)
+
+        c, c8 = ops.KVCache(t(5, 16, 2, 64), t(5, 16, 2, 64)), ops.KVCache(
+            *(t(5, 16, 2, 64, dtype=torch.int8) for _ in range(2)), *(t(5, 16, 2, dtype=f32) for _ in range(2)))
+        write, read, v, slots = ops.kv_cache_write, ops.kv_cache_read, t(4, 2, 64), t(4, dtype=i32)
+        refuse(ValueError, "no scales", write, ops.KVCache(c.k, c.v, c8.k_scales, c8.v_scales), k, v, slots)
+        refuse(ValueError, "has scales", write, ops.KVCache(c8.k, c8.v), k, v, slots)
+        refuse(ValueError, "k_scales must be", write, ops.KVCache(c8.k, c8.v, t(5, 16, 3, dtype=f32), c8.v_scales), k, v, slots)
+        refuse(ValueError, "one shape", write, ops.KVCache(c.k, t(5, 16, 2, 32)), k, v, slots)
+        refuse(TypeError, "cache.v", write, ops.KVCache(c.k, c8.v), k, v, slots)
+        refuse(ValueError, "k must be", write, c, t(4, 3, 64), v, slots)
+        refuse(ValueError, "v must be", write, c, k, t(3, 2, 64), slots)
+        refuse(TypeError, "v must be", write, c, k, t(4, 2, 64, dtype=f32), slots)
+        refuse(TypeError, "slots", write, c, k, v, t(4, dtype=f32))
+        refuse(ValueError, "at most 512", write, ops.KVCache(t(5, 16, 2, 520), t(5, 16, 2, 520)), t(4, 2, 520), t(4, 2, 520), slots)
+        refuse(ValueError, "2\\^31", write, ops.KVCache(*(t(1, 1, 2, 64).expand(1 << 20, 1 << 11, 2, 64) for _ in range(2))), k, v, slots)
+        refuse(TypeError, "dtype", read, c8, slots, dtype=torch.int8)
+        refuse(ValueError, "slots must have 1", read, c, t(4, 1, dtype=i32))
+        refuse(TypeError, "dtype", ops.kv_cache, 1, 1, 1, 1, dtype=torch.float64)
+        refuse(ValueError, "positive", ops.kv_cache, 0, 1, 1, 1)
+
+        att, table, lens = ops.paged_attention, t(4, 3, dtype=i32), t(4, dtype=i32)
+        refuse(TypeError, "q must be", att, t(4, 8, 64, dtype=f32), c, table, lens)
+        refuse(TypeError, "does not go with", att, t(4, 8, 64, dtype=torch.float16), c, table, lens)
+        refuse(ValueError, "do not go with", att, t(4, 7, 64), c, table, lens)
+        refuse(ValueError, "do not go with", att, t(4, 8, 32), c, table, lens)
+        refuse(ValueError, "16 bytes", att, t(4, 8, 72), ops.KVCache(*(t(5, 16, 2, 72, dtype=torch.int8) for _ in range(2)), *c8[2:]), table, lens)
+        refuse(ValueError, "at most 256", att, t(4, 8, 264), ops.KVCache(t(5, 16, 2, 264), t(5, 16, 2, 264)), table, lens)
+        refuse(ValueError, "4 rows", att, q, c, t(5, 3, dtype=i32), lens)
+        refuse(ValueError, "4 rows", att, q, c, table, t(3, dtype=i32))
+        refuse(TypeError, "page_table", att, q, c, t(4, 3, dtype=torch.int64), lens)
+        refuse(ValueError, "at least 1", att, q, c, t(4, 0, dtype=i32), lens)
+        refuse(ValueError, "window", att, q, c, table, lens, window=-1)
+        refuse(ValueError, "out must be", att, q, c, table, lens, out=t(4, 8, 32))
+
+        lora, x, y, A, B, ids = ops.lora_add, t(6, 32), t(6, 48), t(3, 8, 32), t(3, 48, 8), t(6, dtype=i32)
+        refuse(ValueError, "go together", lora, y, t(6, 31), A, B, ids)
+        refuse(ValueError, "go together", lora, y, x, A, t(3, 48, 7), ids)
+        refuse(TypeError, "B must be", lora, y, x, A, t(3, 48, 8, dtype=f32), ids)
+        refuse(ValueError, "rank", lora, y, x, t(3, 129, 32), t(3, 48, 129), ids)
+        refuse(ValueError, "contiguous", lora, y, x, t(3, 32, 8).transpose(1, 2), B, ids)
+        refuse(ValueError, "adapters must have", lora, y, x, A, B, t(5, dtype=i32))
+        refuse(TypeError, "scales", lora, y, x, A, B, ids, t(3))
+        refuse(ValueError, "out must be", lora, y, x, A, B, ids, None, t(6, 47))
+        refuse(RuntimeError, "forward only", lora, y, x, A.clone().requires_grad_(), B, ids)
+
+
+def test_launchers_refuse_what_the_kernels_do_not_take(C):
+    """The native entry points check by themselves, before any launch."""
+    k = C.kernels
+    st4, st12, c4 = [64] * 4, [64] * 12, [16] * 4
+    with pytest.raises(ValueError, match="even"):
+        k.qk_norm_rope(16, 16, 16, 16, 0, 0, False, [1] * 8, 4, 2, 2, 7, 2, 16, 0, 16, 0, 2, False, 1e-6, 0)
+    with pytest.raises(ValueError, match="element type"):
+        k.qk_norm_rope(16, 16, 16, 16, 0, 0, False, [1] * 8, 4, 2, 2, 8, 9, 16, 0, 16, 0, 2, False, 1e-6, 0)
+    for fn in (k.kv_cache_write, k.kv_cache_read):
+        with pytest.raises(ValueError, match="scales"):
+            fn([16, 16], st4, 2, [16, 16, 0, 0], st12, 4, 2, 16, 16, 0, 4, 2, 64, 0)
+        with pytest.raises(ValueError, match="dim"):
+            fn([16, 16], st4, 2, c4, st12, 2, 2, 16, 16, 0, 4, 2, 513, 0)
+        with pytest.raises(ValueError, match="sizes"):
+            fn([16, 16], st4, 2, c4, st12, 2, 2, 0, 16, 0, 4, 2, 64, 0)
+    att = [16, 64, 64, 2, c4, st12, 2, 5, 16, 16, 3, 3, 16, 4, 2, 4, 64, 0, 1.0, 16, 0, 16, 1 << 20, 0]
+
+    def changed(i, v):
+        return att[:i] + [v] + att[i + 1:]
+
+    for i, v, match in ((16, 12, "16 bytes"), (4, [8] * 4, "multiples of 16"), (5, [3] * 12, "multiples of 16"), (22, 10, "workspace"),
+                        (13, 0, "sizes"), (11, 0, "sizes"), (7, 0, "sizes"), (8, 0, "sizes"), (11, 1 << 30, "2\\^30")):
+        with pytest.raises(ValueError, match=match):
+            k.paged_attention(*changed(i, v))
+    with pytest.raises(ValueError, match="rank"):
+        k.lora_add(16, 8, 16, 8, 16, 8, 16, 16, 16, 0, 0, 4, 8, 8, 129, 1, 2, 16, 1 << 20, 0)
+    with pytest.raises(ValueError, match="workspace"):
+        k.lora_add(16, 8, 16, 8, 16, 8, 16, 16, 16, 0, 0, 4, 8, 8, 16, 1, 2, 16, 1, 0)
