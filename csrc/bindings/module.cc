@@ -1236,7 +1236,7 @@ PYBIND11_MODULE(_C, m) {
     a.A = P<const void>(A), a.B = P<const void>(B);
     a.ids = P<const void>(ids), a.ids64 = ids64, a.scales = P<const float>(scales);
     a.rows = rows, a.inner = int(inner), a.outer = int(outer), a.rank = int(rank), a.adapters = int(adapters), a.type = type;
-    if (rows > 0 && kern::lora_workspace(rows, a.inner, a.rank) > ws_floats)
+    if (rows > 0 && kern::lora_workspace(rows, a.inner, a.rank, a.adapters) > ws_floats)
       throw std::invalid_argument("lora_add: workspace too small");
     a.h = P<float>(ws);
     kern::lora_add(a, as_stream(s));

@@ -90,18 +90,29 @@ __device__ __forceinline__ float to_memory(float x, int lane) {
   return __uint_as_float(from_lane(__float_as_uint(x), (lane & 3) * 16 + (lane >> 2)));
 }
 
+__device__ __forceinline__ int adapter_of(const LoraArgs& a, int64_t row) {
+  const int64_t v = load_index(a.ids, a.ids64, row);
+  return v >= 0 && v < a.adapters ? int(v) : -1;
+}
+
 // The rows of a workgroup by adapter; every wave has them alike.  A lane holds its
 // row's adapter and the set of rows that share it, found bit by bit of the adapter's
 // number: walking the groups one after the other, a ballot each, took longer than the
 // products of a mixed batch (16 groups: 4 us of 8).
 struct Groups {
-  int id;          // of this lane's row, -1: none
+  int row;         // of x, y and out: this lane's
+  int id;          // its adapter, -1: none
   uint64_t peers;  // rows of the same adapter
   uint64_t rest;   // the first row of each group that is still to come
   __device__ Groups(const LoraArgs& a, int64_t row0, int rows, int lane) {
-    int64_t v = -1;
-    if (lane < rows && row0 + lane < a.rows) v = load_index(a.ids, a.ids64, row0 + lane);
-    id = v >= 0 && v < a.adapters ? int(v) : -1;
+    const bool is = lane < rows && row0 + lane < a.rows;
+    row = int(row0) + lane;
+    id = -1;
+    if (a.order && !*a.grouped) {
+      if (is) row = a.order[row0 + lane].x, id = a.order[row0 + lane].y;
+    } else if (is) {
+      id = adapter_of(a, row0 + lane);
+    }
     peers = __ballot(id >= 0);
     for (int bit = 0; (a.adapters - 1) >> bit; ++bit) {
       const bool mine = id >> bit & 1;
@@ -137,6 +148,99 @@ __device__ __forceinline__ int share(int n, int waves) {
   return waves == 4 && log2 == 3 ? 2 : log2;
 }
 
+// ---- the rows of a large batch in the order of their adapters
+// One workgroup's stable counting sort: a prompt's 64-row workgroups read an adapter once for all of its rows, and
+// with the rows mixed each would hold a few of every adapter (8192 rows, 32 adapters: 277 us).  Rows that already lie
+// in runs are left: then only the flag is written.  16 waves take a stretch of the rows each and count its adapters in
+// counters of their own, so the order, and with it every sum's, is the same each time.
+constexpr int kSortWaves = 16, kSortThreads = 64 * kSortWaves, kSortAdapters = 2000;
+__global__ __launch_bounds__(kSortThreads) void lora_sort(const LoraArgs a) {
+  extern __shared__ int counts[];  // [kSortWaves][adapters + 1]: the last for rows without one
+  __shared__ int sums[kSortWaves];
+  const int wave = wave_number(), lane = threadIdx.x & 63, n = a.adapters + 1, rows = int(a.rows);
+  const auto block_scan = [&](int x, int& total) {  // the sum of the threads in front
+    int sc = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(sc, o);
+      sc += lane >= o ? y : 0;
+    }
+    if (lane == 63) sums[wave] = sc;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      if (w < wave) before += sums[w];
+      total += sums[w];
+    }
+    __syncthreads();
+    return before + sc - x;
+  };
+  int changes = 0, total;
+#pragma unroll 8
+  for (int t = threadIdx.x; t < rows; t += kSortThreads) changes += adapter_of(a, t) != adapter_of(a, t > 0 ? t - 1 : 0);
+  block_scan(changes, total);
+  const bool grouped = total <= rows / 64;
+  if (threadIdx.x == 0) *a.grouped = grouped;
+  if (grouped) return;  // the whole workgroup
+
+  for (int i = threadIdx.x; i < kSortWaves * n; i += kSortThreads) counts[i] = 0;
+  __syncthreads();
+  int* const mine = counts + wave * n;
+  const int stretch = (rows + 64 * kSortWaves - 1) / (64 * kSortWaves) * 64;
+  const int r0 = min(rows, wave * stretch), r1 = min(rows, r0 + stretch);
+  // 64 rows of the stretch: this lane's adapter (`adapters` for none, -1 behind the stretch) and the lanes with the same
+  const auto chunk = [&](int t, int& id, uint64_t& peers) {
+    id = -1;
+    if (t < r1) {
+      id = adapter_of(a, t);
+      if (id < 0) id = a.adapters;
+    }
+    peers = __ballot(id >= 0);
+    for (int bit = 0; a.adapters >> bit; ++bit) {
+      const bool set = id >> bit & 1;
+      const uint64_t with = __ballot(set);
+      peers &= set ? with : ~with;
+    }
+    return id >= 0 && __builtin_ctzll(peers) == lane;
+  };
+  for (int t = r0; t < r1; t += 64) {
+    int id;
+    uint64_t peers;
+    if (chunk(t + lane, id, peers)) mine[id] += __popcll(peers);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  // each counter becomes the place of its first row: adapters in their order, each one's waves in theirs
+  const int entries = kSortWaves * n, each = (entries + kSortThreads - 1) / kSortThreads;
+  const int e0 = min(entries, int(threadIdx.x) * each), e1 = min(entries, e0 + each);
+  int sum = 0;
+  for (int e = e0; e < e1; ++e) sum += counts[e % kSortWaves * n + e / kSortWaves];
+  int place = block_scan(sum, total);
+  for (int e = e0; e < e1; ++e) {
+    int& c = counts[e % kSortWaves * n + e / kSortWaves];
+    const int x = c;
+    c = place;
+    place += x;
+  }
+  __syncthreads();
+  for (int t = r0; t < r1; t += 64) {
+    int id;
+    uint64_t peers;
+    const bool first = chunk(t + lane, id, peers);
+    int at = 0;
+    if (id >= 0) at = mine[id] + __popcll(peers & ((uint64_t(1) << lane) - 1));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (first) mine[id] += __popcll(peers);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (id >= 0) a.order[at] = make_int2(t + lane, id < a.adapters ? id : -1);
+  }
+}
+
 // ---- h[split][row][rank] = sum over the split's part of the inner dimension
 // NR: rank tiles of 16, ROWS: of a workgroup.
 template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWaves<ROWS>) void lora_down(const LoraArgs a) {
@@ -169,7 +273,7 @@ template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWave
     for (int c = 0; c < CT; ++c) {
       // a column behind the group's last row takes its first row again, and is not stored
       const int at = __shfl(place, c * 16 + row < count ? c * 16 + row : 0);
-      xr[c] = static_cast<const T*>(a.x) + (row0 + at) * a.x_row + run;
+      xr[c] = static_cast<const T*>(a.x) + __shfl(groups.row, at) * a.x_row + run;
     }
 #pragma unroll
     for (int r = 0; r < NR; ++r) Ar[r] = A + int64_t(min(r * 16 + row, a.rank - 1)) * a.inner;
@@ -304,7 +408,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
   // product tile n is column 4 kRun (n / kPairs) + kRun (i / 4) + 4 (n % kPairs) + i % 4.
   constexpr int kPer = 16 / kRun<T>, kPairs = kRun<T> / 4;
   struct Piece {
-    int tile, count, at[NC];
+    int tile, count, at[NC], row[NC];
     frag<T> b[4][KS], y[NC][kPer];
   };
   const uint64_t all_groups = groups.rest;
@@ -336,7 +440,8 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
     for (int c = 0; c < NC; ++c) {
       // a row behind the group's last is its first again, and is not stored
       w.at[c] = __shfl(place, c * 16 + row < count ? c * 16 + row : 0);
-      const T* const y = static_cast<const T*>(a.y) + (row0 + w.at[c]) * a.y_row + col;
+      w.row[c] = __shfl(groups.row, w.at[c]);
+      const T* const y = static_cast<const T*>(a.y) + w.row[c] * a.y_row + col;
 #pragma unroll
       for (int q = 0; q < kPer; ++q) {
         if constexpr (decltype(full)::value) w.y[c][q] = load_any<frag<T>>(y + q * 4 * kRun<T>);
@@ -394,7 +499,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
           v[q][j] = float(w.y[c][q][j]) + (kExchange ? to_memory(x, lane) : x);
         }
       if (c * 16 + row < w.count) {
-        T* const out = static_cast<T*>(a.out) + (row0 + w.at[c]) * a.out_row + col;
+        T* const out = static_cast<T*>(a.out) + w.row[c] * a.out_row + col;
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
           const int left = a.outer - col - q * 4 * kRun<T>;
@@ -498,8 +603,9 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
   const int col0 = tile0 * 64, cols = min(a.outer, tile1 * 64) - col0;
   for (int row = 0; row < ROWS && row0 + row < a.rows; ++row) {
     if (valid >> row & 1) continue;
-    const T* const y = static_cast<const T*>(a.y) + (row0 + row) * a.y_row + col0;
-    T* const out = static_cast<T*>(a.out) + (row0 + row) * a.out_row + col0;
+    const int64_t at = __builtin_amdgcn_readlane(groups.row, row);
+    const T* const y = static_cast<const T*>(a.y) + at * a.y_row + col0;
+    T* const out = static_cast<T*>(a.out) + at * a.out_row + col0;
     for (int i = threadIdx.x * kRun<T>; i < cols; i += kThreads * kRun<T>) {
       if (i + kRun<T> <= cols) store_any(out + i, load_any<frag<T>>(y + i));
       else
@@ -510,9 +616,11 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
 
 int rank_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 // Few rows: 4 of a workgroup, so that each adapter of a mixed batch has a wave of its own (16 rows with 16 waves took
-// twice as long: one workgroup a CU, and all its waves wait for the same things).  Many: 32 or 64, which read an adapter
-// once for all of them.
-bool few(int64_t rows) { return rows <= 1024; }
+// twice as long: one workgroup a CU, and all its waves wait for the same things).  Many: 32 or 64, sorted by adapter,
+// which read it once for all of them.  The more ranks, the sooner the second pays (4096 -> 4096, few against many, rows
+// in runs of 4 adapters / mixed over 32: 512 rows of rank 16 12 : 19 / 26 : 20 us, 1000 rows 20 : 21 / 40 : 25; 200 rows
+// of rank 64 18 : 23 / 48 : 31 us, 1000 rows 45 : 25 / 107 : 31).
+bool few(int64_t rows, int rank) { return rows * 16 * rank_tiles(rank) <= 8192; }
 
 template <class T, int NR, int ROWS> void down(const LoraArgs& a, hipStream_t s) {
   const dim3 grid(unsigned((a.rows + ROWS - 1) / ROWS), unsigned(a.splits));
@@ -530,7 +638,7 @@ template <class T, int KS, int ROWS> void up(const LoraArgs& a, hipStream_t s) {
 
 template <class T, int NR> void both(const LoraArgs& a, hipStream_t s) {
   constexpr int KS = (16 * NR + kDeep<T> - 1) / kDeep<T>;
-  if (few(a.rows)) {
+  if (few(a.rows, a.rank)) {
     down<T, NR, 4>(a, s);
     up<T, KS, 4>(a, s);
   } else {
@@ -548,17 +656,21 @@ template <class T> void dispatch(const LoraArgs& a, hipStream_t s) {
   }
 }
 
-int splits_of(int64_t rows, int inner) {
+// Whether rows are sorted first: 64 of a workgroup gain by it, and the counters have to fit in LDS.
+bool sorts(int64_t rows, int rank, int adapters) { return !few(rows, rank) && adapters > 1 && adapters <= kSortAdapters; }
+
+int splits_of(int64_t rows, int inner, int rank) {
   // about two workgroups of four waves (one of eight) for each CU, of 256 (512) of the inner dimension or more
-  const int64_t want = few(rows) ? 2048 / rows : 8192 / rows, most = inner / (few(rows) ? 256 : 512);
+  const bool small = few(rows, rank);
+  const int64_t want = (small ? 2048 : 8192) / rows, most = inner / (small ? 256 : 512);
   const int64_t n = want < most ? want : most;
   return int(n < 1 ? 1 : n);
 }
 
 }  // namespace
 
-int64_t lora_workspace(int64_t rows, int inner, int rank) {
-  return int64_t(splits_of(rows, inner)) * rows * 16 * rank_tiles(rank);
+int64_t lora_workspace(int64_t rows, int inner, int rank, int adapters) {
+  return int64_t(splits_of(rows, inner, rank)) * rows * 16 * rank_tiles(rank) + (sorts(rows, rank, adapters) ? 4 + 2 * rows : 0);
 }
 
 void lora_add(LoraArgs a, hipStream_t s) {
@@ -566,12 +678,17 @@ void lora_add(LoraArgs a, hipStream_t s) {
   if (a.inner < 1 || a.outer < 1 || a.adapters < 1 || a.inner > 1 << 24 || a.outer > 1 << 24)
     throw std::invalid_argument("lora_add: sizes");
   if (a.rows <= 0) return;
-  if (a.rows > int64_t(1) << 31) throw std::invalid_argument("lora_add: too many rows for one call");
-  a.splits = splits_of(a.rows, a.inner);
+  if (a.rows > 0x7fffff00) throw std::invalid_argument("lora_add: too many rows for one call");
+  a.splits = splits_of(a.rows, a.inner, a.rank);
+  if (sorts(a.rows, a.rank, a.adapters)) {  // behind h: the flag, then the order
+    a.grouped = reinterpret_cast<int*>(a.h + int64_t(a.splits) * a.rows * 16 * rank_tiles(a.rank));
+    a.order = reinterpret_cast<int2*>(a.grouped + 4);
+    launch_kernel(lora_sort, 1, kSortThreads, size_t(kSortWaves) * (a.adapters + 1) * sizeof(int), s, a);
+  }
   // Columns of a workgroup of "up", in tiles of 64: as few as give the chip four workgroups a CU (two of the larger),
   // since a mixed batch's groups take them one after the other; at most 16.
   const int64_t tiles = (a.outer + 63) / 64;
-  const int64_t each = few(a.rows) ? ((a.rows + 3) / 4 * tiles + 1023) / 1024 : ((a.rows + 63) / 64 * tiles + 511) / 512;
+  const int64_t each = few(a.rows, a.rank) ? ((a.rows + 3) / 4 * tiles + 1023) / 1024 : ((a.rows + 63) / 64 * tiles + 511) / 512;
   a.col_tiles = int(each > 16 ? 16 : each);
   switch (a.type) {
     case kF32: return dispatch<float>(a, s);

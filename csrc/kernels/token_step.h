@@ -8,6 +8,7 @@
 #pragma once
 
 #include <hip/hip_runtime_api.h>
+#include <hip/hip_vector_types.h>
 
 #include <cstdint>
 
@@ -127,8 +128,10 @@ struct LoraArgs {
   float* h = nullptr;           // workspace of lora_workspace() floats
   // filled in by lora_add()
   int splits = 1, col_tiles = 1;
+  int* grouped = nullptr;       // in the workspace: whether the rows lie in runs already
+  int2* order = nullptr;        // else {row, adapter} sorted by adapter; null: never sorted
 };
-int64_t lora_workspace(int64_t rows, int inner, int rank);
+int64_t lora_workspace(int64_t rows, int inner, int rank, int adapters);
 void lora_add(LoraArgs a, hipStream_t stream);
 
 }  // namespace sca::kern

@@ -377,7 +377,7 @@ def lora_add(y, x, A, B, adapters, scales=None, out=None):
     if T and M:
         if _lora_workspace is None:
             _lora_workspace = functools.lru_cache(maxsize=1024)(_k().lora_workspace)
-        n = _lora_workspace(T, K, r)
+        n = _lora_workspace(T, K, r, N)
         ws = torch.empty(n, dtype=torch.float32, device=dev)
         _launch(y, _k().lora_add, y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0),
                 A.data_ptr(), B.data_ptr(), adapters.data_ptr(), _INDEX[adapters.dtype],

@@ -383,7 +383,8 @@ LORA = [  # rows, inner, outer, rank, adapters, mixed
     (1, 1, 1, 1, 1, True), (1, 4096, 4096, 16, 4, True), (64, 1024, 640, 16, 32, True), (17, 200, 77, 12, 3, True),
     (333, 1001, 503, 9, 5, False), (16, 512, 512, 64, 16, True), (40, 300, 1030, 100, 2, False), (5, 4104, 72, 128, 5, True),
     (1025, 512, 384, 8, 3, False), (1100, 320, 200, 32, 40, True), (2000, 264, 1100, 64, 7, False), (1030, 130, 66, 128, 2, True),
-    (1024, 64, 64, 33, 1000, True), (3, 8200, 64, 5, 2, True)]
+    (1024, 64, 64, 33, 1000, True), (3, 8200, 64, 5, 2, True),
+    (4099, 72, 80, 8, 300, True), (1025, 32, 16, 4, 2000, True), (1026, 40, 24, 4, 2001, True), (1100, 33, 17, 4, 1, True)]
 
 
 @pytest.mark.gpu
@@ -419,7 +420,7 @@ def test_lora_add(case, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [6, 1500])
+@pytest.mark.parametrize("T", [6, 512, 513, 1500])
 def test_lora_add_strides_in_place_and_index_types(T):
     """A part of a fused projection changed in place, and its neighbours left as they were."""
     g = gen(T)
