@@ -68,6 +68,17 @@ template <class T> __device__ __forceinline__ frag<T> load_edge(const T* p, int 
   return x;
 }
 
+// The same for a row that ends inside a run, without a branch: `keep` elements from base[off], zeros behind them.  What
+// lies behind is the next row, except at the tensor's end: there the run before `last`, its last one, is shifted.
+template <class T> __device__ __forceinline__ frag<T> load_masked(const T* base, int64_t off, int64_t last, int keep) {
+  using Bits = unsigned __int128;
+  const int64_t from = off < last ? off : last;
+  Bits x = load_any<Bits>(base + from) >> (int(off - from) * int(8 * sizeof(T)) & 127);
+  const Bits mask = keep >= kRun<T> ? ~Bits(0) : keep > 0 ? (Bits(1) << (keep * int(8 * sizeof(T)) & 127)) - 1 : Bits(0);
+  x &= mask;
+  return __builtin_bit_cast(frag<T>, x);
+}
+
 // Memory and the matrix instruction want a wave's 16 rows in different lanes.  A load or store serves 16 neighbouring
 // lanes at a time, one cache access for each row among them, so memory has four lanes side by side on a row (lane =
 // 4 row + run); an operand has its rows side by side (lane = 16 run + row).  Loaded in the operand's order the cache's
@@ -411,6 +422,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
     int tile, count, at[NC], row[NC];
     frag<T> b[4][KS], y[NC][kPer];
   };
+  const int64_t b_last = int64_t(a.adapters) * a.outer * a.rank - kRun<T>;  // where B's last run starts
   const uint64_t all_groups = groups.rest;
   int adapter = 0, turn = 0, place = 0, count = 0, tile = 0, lo = 0, hi = 0;  // tiles lo .. hi - 1 of this turn
   const auto next = [&]() {
@@ -458,6 +470,9 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
         if constexpr (EVEN) {
           w.b[n][k] = load_any<frag<T>>(Bm + (r < a.rank ? r : 0));
           if (r >= a.rank) w.b[n][k] = {};
+        } else if constexpr (decltype(full)::value) {
+          const int from = r < a.rank ? r : 0;
+          w.b[n][k] = load_masked<T>(static_cast<const T*>(a.B), Bm - static_cast<const T*>(a.B) + from, b_last, a.rank - r);
         } else {
           w.b[n][k] = load_edge<T>(Bm, r, a.rank);
         }
@@ -516,7 +531,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
   };
 
   // The full tiles.  The first piece's loads go out before h is known.
-  const int tile_full = min(tile1, a.outer / 64);
+  const int tile_full = EVEN || b_last >= 0 ? max(tile0, min(tile1, a.outer / 64)) : tile0;
   lo = tile0, hi = tile_full, tile = hi;
   bool more = next();
   Piece now;
@@ -599,17 +614,29 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
     }
   }
   if (a.out == a.y) return;
-  // rows without an adapter
-  const int col0 = tile0 * 64, cols = min(a.outer, tile1 * 64) - col0;
-  for (int row = 0; row < ROWS && row0 + row < a.rows; ++row) {
-    if (valid >> row & 1) continue;
-    const int64_t at = __builtin_amdgcn_readlane(groups.row, row);
-    const T* const y = static_cast<const T*>(a.y) + at * a.y_row + col0;
-    T* const out = static_cast<T*>(a.out) + at * a.out_row + col0;
-    for (int i = threadIdx.x * kRun<T>; i < cols; i += kThreads * kRun<T>) {
-      if (i + kRun<T> <= cols) store_any(out + i, load_any<frag<T>>(y + i));
+  // rows without an adapter: four runs of each thread at a time, since a sorted batch has whole workgroups of them
+  const int col0 = tile0 * 64, cols = min(a.outer, tile1 * 64) - col0, runs = (cols + kRun<T> - 1) / kRun<T>;
+  if (!~(valid | (ROWS < 64 ? ~uint64_t(0) << (ROWS & 63) : 0))) return;
+  for (int i0 = 0; i0 < ROWS * runs; i0 += 4 * kThreads) {  // as often for every lane: they exchange rows
+    frag<T> x[4];
+    int64_t at[4];
+    int left[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * kThreads + int(threadIdx.x), row = min(i / runs, ROWS - 1), run = (i - i / runs * runs) * kRun<T>;
+      at[u] = __builtin_amdgcn_ds_bpermute(row * 4, groups.row);
+      left[u] = i < ROWS * runs && row0 + row < a.rows && !(valid >> row & 1) ? cols - run : 0;
+      if (left[u] > 0) x[u] = load_edge<T>(static_cast<const T*>(a.y) + at[u] * a.y_row + col0 + run, 0, left[u]);
+      at[u] = at[u] * a.out_row + col0 + run;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      T* const out = static_cast<T*>(a.out) + at[u];
+      if (left[u] >= kRun<T>) store_any(out, x[u]);
       else
-        for (int j = i; j < cols; ++j) out[j] = y[j];
+#pragma unroll
+        for (int j = 0; j < kRun<T> - 1; ++j)
+          if (j < left[u]) out[j] = x[u][j];
     }
   }
 }
