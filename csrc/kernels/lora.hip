@@ -470,7 +470,7 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
         if constexpr (EVEN) {
           w.b[n][k] = load_any<frag<T>>(Bm + (r < a.rank ? r : 0));
           if (r >= a.rank) w.b[n][k] = {};
-        } else if constexpr (decltype(full)::value) {
+        } else if constexpr (decltype(full)::value && kExchange) {  // of few rows there is no next load to wait for
           const int from = r < a.rank ? r : 0;
           w.b[n][k] = load_masked<T>(static_cast<const T*>(a.B), Bm - static_cast<const T*>(a.B) + from, b_last, a.rank - r);
         } else {
@@ -614,9 +614,22 @@ __global__ __launch_bounds__(kThreads) void lora_up(const LoraArgs a, int ranks)
     }
   }
   if (a.out == a.y) return;
-  // rows without an adapter: four runs of each thread at a time, since a sorted batch has whole workgroups of them
+  // Rows without an adapter.
   const int col0 = tile0 * 64, cols = min(a.outer, tile1 * 64) - col0, runs = (cols + kRun<T> - 1) / kRun<T>;
-  if (!~(valid | (ROWS < 64 ? ~uint64_t(0) << (ROWS & 63) : 0))) return;
+  if constexpr (ROWS == kWaves) {  // one for each wave
+    if (row0 + wave >= a.rows || (valid >> wave & 1)) return;
+    const int64_t at = row0 + wave;
+    for (int i = lane * kRun<T>; i < cols; i += 64 * kRun<T>) {
+      const T* const y = static_cast<const T*>(a.y) + at * a.y_row + col0 + i;
+      T* const out = static_cast<T*>(a.out) + at * a.out_row + col0 + i;
+      if (i + kRun<T> <= cols) store_any(out, load_any<frag<T>>(y));
+      else
+        for (int j = 0; j < cols - i; ++j) out[j] = y[j];
+    }
+    return;
+  }
+  // A sorted batch has whole workgroups of them: four runs of each thread at a time.
+  if (!~valid) return;
   for (int i0 = 0; i0 < ROWS * runs; i0 += 4 * kThreads) {  // as often for every lane: they exchange rows
     frag<T> x[4];
     int64_t at[4];

@@ -288,7 +288,8 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
     of 8, of 16 with 8 bits), starting at one.  A length beyond the table counts
     as the table's end, a negative one as 0; tokens on a page outside the cache
     are left out, and what the cache holds where nothing is seen (anything, NaN
-    too) does not matter.  A request that sees nothing gets zeros.
+    too) does not matter.  A request that sees nothing gets zeros.  A value that
+    is seen and is infinite or NaN makes its dimension NaN.
 
     Returns [B, Hq, D] in q's type (``out`` if given: contiguous, not
     overlapping q), with ``return_lse`` also the natural logsumexp of its scores
@@ -301,7 +302,7 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
     pages, page, H, dim = c.shape
     if c.dtype.itemsize != 1 and c.dtype != q.dtype:
         raise TypeError(f"a cache of {c.dtype} does not go with queries of {q.dtype}")
-    if dim != D or Hq % H or not Hq:
+    if dim != D or not H or not Hq or Hq % H:
         raise ValueError(f"queries {tuple(q.shape)} do not go with a cache of {H} heads of {dim}")
     if D > 256 or D * c.dtype.itemsize % 16:
         raise ValueError(f"dim must be at most 256 and fill multiples of 16 bytes in the cache, got {D} of {c.dtype}")
@@ -346,8 +347,8 @@ def lora_add(y, x, A, B, adapters, scales=None, out=None):
     negative or behind the last keeps y.  Rows may come in any order; many rows
     are fastest where those of one adapter lie together.
 
-    Sums are fp32, with one rounding at the end.  Returns a new tensor, or
-    ``out``, which may be ``y`` itself (other overlaps are not allowed).
+    Sums are fp32, with one rounding at the end; an infinite weight of B gives
+    NaN.  Returns a new tensor, or ``out``, which may be ``y`` itself (other overlaps are not allowed).
     """
     global _lora_workspace
     _tensor(y, "y", 2, _FLOATS)

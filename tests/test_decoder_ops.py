@@ -663,6 +663,7 @@ def test_refusals_before_anything_is_launched():
         refuse(TypeError, "does not go with", att, t(4, 8, 64, dtype=torch.float16), c, table, lens)
         refuse(ValueError, "do not go with", att, t(4, 7, 64), c, table, lens)
         refuse(ValueError, "do not go with", att, t(4, 8, 32), c, table, lens)
+        refuse(ValueError, "do not go with", att, q, ops.KVCache(t(5, 16, 0, 64), t(5, 16, 0, 64)), table, lens)
         refuse(ValueError, "16 bytes", att, t(4, 8, 72), ops.KVCache(*(t(5, 16, 2, 72, dtype=torch.int8) for _ in range(2)), *c8[2:]), table, lens)
         refuse(ValueError, "at most 256", att, t(4, 8, 264), ops.KVCache(t(5, 16, 2, 264), t(5, 16, 2, 264)), table, lens)
         refuse(ValueError, "4 rows", att, q, c, t(5, 3, dtype=i32), lens)
