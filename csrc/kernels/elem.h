@@ -128,8 +128,12 @@ __device__ __forceinline__ float group_max(float v, int width) {
   return v;
 }
 
+// An int32 or int64 (is64 is 0 or 1), as two words and without a branch between the two, which would keep a loop's loads
+// from being under way together.
 __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i) {
-  return is64 ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
+  const int32_t* const words = static_cast<const int32_t*>(p) + (i << is64);
+  const int32_t low = words[0], high = words[is64];
+  return int64_t(is64 ? high : low >> 31) << 32 | uint32_t(low);
 }
 
 }  // namespace sca::kern

@@ -7,13 +7,12 @@
 // fraction of what the matrix cores do in that time, so both are bound by memory,
 // and with few rows by the latency of a few dependent loads.
 //
-// The rows of a workgroup are sorted into groups of one adapter by ballots, in
-// registers: no plan is made on the host and no order is asked of the caller.  A
-// group of up to 16 rows is one column tile of the matrix instruction, whatever
-// the adapter's other rows are, so x and y are touched once however the rows are
-// mixed.  The four waves of a workgroup share the groups; where there are fewer
-// than four (a prompt's rows), the waves that are left split the inner dimension
-// (down) or the columns (up).
+// The rows of a workgroup are put into groups of one adapter by ballots, in registers;
+// a large batch whose rows are mixed is first put in its adapters' order by lora_sort.
+// No plan is made on the host and no order is asked of the caller.  A group's rows are
+// columns of the matrix instruction, 16 at a time, and x and y are touched once.  The
+// waves of a workgroup share the groups; where there are fewer groups than waves, those
+// left split the inner dimension (down) or the columns (up).
 //
 // Down splits the inner dimension over workgroups too while the rows alone would
 // not fill the chip; its partial sums are added in their order by up, so nothing is
@@ -21,6 +20,9 @@
 // the sum of two 16-bit numbers (high part and remainder): rounding h once would
 // cost as much as the output's own rounding.  fp16 has it over the row's largest
 // power of two, which is multiplied back in fp32, so that it cannot overflow.
+//
+// 4096 to 4096 in bf16: 64 rows of 32 adapters of rank 16 take 5.2 + 6.0 us (two chains of waits); 8192 rows of 8
+// adapters of rank 64 take 4.7 (is it sorted?) + 26 + 34 us for 210 MB.
 #include <hip/hip_runtime.h>
 
 #include <stdexcept>
