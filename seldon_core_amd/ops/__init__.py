@@ -11,10 +11,26 @@ operators of served token models are in :mod:`.token_step`.
 """
 from __future__ import annotations
 
+import importlib
 from typing import List, Sequence
 
 from .._native import native
-from .token_step import KVCache, kv_cache, kv_cache_read, kv_cache_write, lora_add, paged_attention, qk_norm_rope  # noqa: F401
+
+_TOKEN_STEP = ("KVCache", "kv_cache", "kv_cache_read", "kv_cache_write", "lora_add", "paged_attention", "qk_norm_rope")
+
+
+def __getattr__(name):
+    # token_step loads torch (1.5 s), which the CPU references here do without: only where it is asked for
+    if name == "token_step":
+        return importlib.import_module(".token_step", __name__)
+    if name in _TOKEN_STEP:
+        value = globals()[name] = getattr(importlib.import_module(".token_step", __name__), name)
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted({*globals(), *_TOKEN_STEP, "token_step"})
 
 
 def _k():
