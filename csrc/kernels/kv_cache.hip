@@ -203,10 +203,15 @@ void run(const KvCacheArgs& a, bool write, hipStream_t s) {
   if (a.dim < 1 || a.dim > 512) throw std::invalid_argument("kv_cache: dim is 1 to 512");
   if (a.page.d < 1 || a.slots_total < 0 || a.slots_total > 0x7fffffff)
     throw std::invalid_argument("kv_cache: at most 2^31 - 1 slots, in pages of at least one");
-  if ((a.cache_type == kE4M3 || a.cache_type == kI8) && (!a.scale[0] || !a.scale[1]))
+  if (a.slots_total && (a.cache_type == kE4M3 || a.cache_type == kI8) && (!a.scale[0] || !a.scale[1]))
     throw std::invalid_argument("kv_cache: an 8-bit cache has scales");
   if (a.rows <= 0) return;
   if (a.rows > 0x7fffffff / int64_t(a.heads.d)) throw std::invalid_argument("kv_cache: at most 2^31 - 1 rows times heads");
+  for (int i = 0; i < 2; ++i) {
+    need_memory(a.x[i], "kv_cache: a tensor of rows");
+    if (a.slots_total) need_memory(a.cache[i], "kv_cache: the cache");
+  }
+  need_memory(a.slots, "kv_cache: slots");
   switch (a.type) {
     case kF32: return by_cache<float>(a, write, s);
     case kF16: return by_cache<f16>(a, write, s);

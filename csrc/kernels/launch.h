@@ -10,6 +10,11 @@
 
 namespace sca::kern {
 
+// What a kernel reads or writes has an address: a tensor without memory (a fake one, as tracers use) has none.
+inline void need_memory(const void* p, const char* what) {
+  if (!p) throw std::invalid_argument(std::string(what) + " has no memory");
+}
+
 template <class... P, class... A>
 void launch_kernel(void (*fn)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t s, A&&... args) {
   static_assert(sizeof...(P) == sizeof...(A), "one argument for each parameter");

@@ -721,6 +721,13 @@ void lora_add(LoraArgs a, hipStream_t s) {
     throw std::invalid_argument("lora_add: sizes");
   if (a.rows <= 0) return;
   if (a.rows > 0x7fffff00) throw std::invalid_argument("lora_add: too many rows for one call");
+  need_memory(a.x, "lora_add: x");
+  need_memory(a.y, "lora_add: y");
+  need_memory(a.out, "lora_add: out");
+  need_memory(a.A, "lora_add: A");
+  need_memory(a.B, "lora_add: B");
+  need_memory(a.ids, "lora_add: adapters");
+  need_memory(a.h, "lora_add: the workspace");
   a.splits = splits_of(a.rows, a.inner, a.rank);
   if (sorts(a.rows, a.rank, a.adapters)) {  // behind h: the flag, then the order
     a.grouped = reinterpret_cast<int*>(a.h + int64_t(a.splits) * a.rows * 16 * rank_tiles(a.rank));

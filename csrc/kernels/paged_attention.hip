@@ -615,6 +615,12 @@ int64_t paged_attention_workspace(int batch, int kv_heads, int group, int dim, b
 }
 
 void paged_attention(const PagedAttentionArgs& a, hipStream_t s) {
+  need_memory(a.q, "paged_attention: q");
+  need_memory(a.out, "paged_attention: out");
+  for (const void* c : a.cache) need_memory(c, "paged_attention: the cache");
+  need_memory(a.table, "paged_attention: page_table");
+  need_memory(a.lengths, "paged_attention: lengths");
+  need_memory(a.partial_ml, "paged_attention: the workspace");
   if (a.type == kBF16) return by_cache<bf16>(a, s);
   if (a.type == kF16) return by_cache<f16>(a, s);
   throw std::invalid_argument("paged_attention: queries are fp16 or bf16");

@@ -175,6 +175,13 @@ void qk_norm_rope(const QkNormRopeArgs& a, hipStream_t s) {
   if (a.heads[0] < 0 || a.heads[1] < 0) throw std::invalid_argument("qk_norm_rope: heads");
   if (a.tokens <= 0 || a.heads[0] + a.heads[1] == 0) return;
   if (a.tokens > int64_t(1) << 32) throw std::invalid_argument("qk_norm_rope: too many tokens");
+  for (int i = 0; i < 2; ++i) {
+    if (!a.heads[i]) continue;
+    need_memory(a.x[i], "qk_norm_rope: an input");
+    need_memory(a.out[i], "qk_norm_rope: an output");
+  }
+  need_memory(a.positions, "qk_norm_rope: positions");
+  if (a.n_freq) need_memory(a.inv_freq, "qk_norm_rope: inv_freq");
   switch (a.type) {
     case kF32: return dispatch<float>(a, s);
     case kF16: return dispatch<f16>(a, s);

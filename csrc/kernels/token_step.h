@@ -4,7 +4,8 @@
 // Like the others (kernels.h) they are asynchronous on `stream`, allocate
 // nothing and never synchronise.  Strides count elements; the last dimension of
 // every tensor is contiguous.  They throw std::invalid_argument for what they do
-// not take and std::runtime_error for a launch that fails.
+// not take (a null pointer that is not called optional among it) and
+// std::runtime_error for a launch that fails.
 #pragma once
 
 #include <hip/hip_runtime_api.h>

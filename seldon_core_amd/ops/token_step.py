@@ -14,8 +14,8 @@ Every op launches hand-written HIP kernels on the current stream of its
 tensors' device, allocates only its outputs and workspace (from torch's
 allocator, so a captured graph keeps its own) and never synchronises: lengths,
 page tables, slots and adapter ids are read on the GPU only.  What the host can
-see (shapes, types, strides, devices) is checked and refused with
-``ValueError`` / ``TypeError``; indices that point outside a cache or a table
+see (shapes, types, strides, devices, tensors without memory, as tracers use
+them) is checked and refused with ``ValueError`` / ``TypeError``; indices that point outside a cache or a table
 are left out by the kernels as each op says.  The ops are forward only.
 
 Kernel sources: csrc/kernels/{rope,kv_cache,paged_attention,lora}.hip.
@@ -84,6 +84,16 @@ def _launch(t, fn, *args):
             fn(*args, _stream_of(index))
 
 
+def _optional(t, name):
+    """The address of a tensor that may be None: 0 for None only (the kernels refuse a null pointer elsewhere)."""
+    if t is None:
+        return 0
+    p = t.data_ptr()
+    if not p and t.numel():
+        raise ValueError(f"{name} has no memory")
+    return p
+
+
 def _new(t):
     """An uninitialised contiguous tensor of t's shape, type and device."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
@@ -142,7 +152,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, *, eps: float = 
                 raise ValueError(f"{name} must be {tuple(x.shape)}, got {tuple(o.shape)}")
     if T and Hq + Hk:
         _launch(q, _k().qk_norm_rope, q.data_ptr(), k.data_ptr(), oq.data_ptr(), ok.data_ptr(),
-                0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), bool(wf32),
+                _optional(q_weight, "q_weight"), _optional(k_weight, "k_weight"), bool(wf32),
                 q.stride()[:2] + k.stride()[:2] + oq.stride()[:2] + ok.stride()[:2], T, Hq, Hk, D, _TYPE[dt],
                 positions.data_ptr(), _INDEX[positions.dtype], inv_freq.data_ptr(), inv_freq.dtype == torch.float64,
                 inv_freq.shape[0], interleaved, eps)
@@ -382,7 +392,7 @@ def lora_add(y, x, A, B, adapters, scales=None, out=None):
         ws = torch.empty(n, dtype=torch.float32, device=dev)
         _launch(y, _k().lora_add, y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0),
                 A.data_ptr(), B.data_ptr(), adapters.data_ptr(), _INDEX[adapters.dtype],
-                0 if scales is None else scales.data_ptr(), T, K, M, r, N, _TYPE[dt], ws.data_ptr(), n)
+                _optional(scales, "scales"), T, K, M, r, N, _TYPE[dt], ws.data_ptr(), n)
     return out
 
 

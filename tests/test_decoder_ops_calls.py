@@ -23,3 +23,76 @@ def test_importing_ops_does_not_load_torch():
             "try:\n    ops.no_such_op\nexcept AttributeError:\n    print('fine')\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip() == "fine", r.stderr
+
+
+# ---------------------------------------------------------------- refusals
+@pytest.fixture
+def no_device(monkeypatch):
+    """Calls get as far as the native launchers, which refuse before they launch, on a machine without a GPU too."""
+    monkeypatch.setattr(ops.token_step, "_stream_of", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+
+
+def fake(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="cuda")
+
+
+def fake_calls(dtype=torch.bfloat16):
+    """One call of each operator on tensors that take part in nothing, as (name, function)."""
+    i32, f32, c8 = torch.int32, torch.float32, torch.int8
+    q, k, table, n = fake(4, 8, 64, dtype=dtype), fake(4, 2, 64, dtype=dtype), fake(4, 3, dtype=i32), fake(4, dtype=i32)
+    cache = ops.KVCache(fake(5, 16, 2, 64, dtype=dtype), fake(5, 16, 2, 64, dtype=dtype))
+    eight = ops.KVCache(*(fake(5, 16, 2, 64, dtype=c8) for _ in range(2)), *(fake(5, 16, 2, dtype=f32) for _ in range(2)))
+    x, y, A, B = fake(6, 32, dtype=dtype), fake(6, 48, dtype=dtype), fake(3, 8, 32, dtype=dtype), fake(3, 48, 8, dtype=dtype)
+    return {
+        "rope": lambda: ops.qk_norm_rope(q, k, None, None, n, fake(32, dtype=f32)),
+        "write": lambda: ops.kv_cache_write(cache, k, k.clone(), n),
+        "write 8": lambda: ops.kv_cache_write(eight, k, k.clone(), n),
+        "read": lambda: ops.kv_cache_read(cache, n),
+        "read 8": lambda: ops.kv_cache_read(eight, n),
+        "attention": lambda: ops.paged_attention(q, cache, table, n, return_lse=True),
+        "attention 8": lambda: ops.paged_attention(q, eight, table, n),
+        "lora": lambda: ops.lora_add(y, x, A, B, fake(6, dtype=i32), fake(3, dtype=f32)),
+    }
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+@pytest.mark.parametrize("op", ["rope", "write", "write 8", "read", "read 8", "attention", "attention 8", "lora"])
+def test_fake_tensors_are_refused(op, no_device):
+    """Every check of shapes and types holds for a fake tensor, whose address is 0: no kernel may be given it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        call = fake_calls()[op]
+        with pytest.raises(ValueError, match="no memory|has scales"):
+            call()
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+def test_a_fake_weight_is_not_taken_for_none():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        w = fake(64)
+    assert ops.token_step._optional(None, "w") == 0
+    with pytest.raises(ValueError, match="w has no memory"):
+        ops.token_step._optional(w, "w")
+
+
+def test_launchers_refuse_null_pointers(C):
+    k = C.kernels
+    st4, st12, c4 = [64] * 4, [64] * 12, [16] * 4
+    rope = [16, 16, 16, 16, 0, 0, False, [1] * 8, 4, 2, 2, 8, 2, 16, 0, 16, 0, 2, False, 1e-6, 0]
+    cache = [[16, 16], st4, 2, c4, st12, 2, 2, 16, 16, 0, 4, 2, 64, 0]
+    att = [16, 64, 64, 2, c4, st12, 2, 5, 16, 16, 3, 3, 16, 4, 2, 4, 64, 0, 1.0, 16, 0, 16, 1 << 20, 0]
+    lora = [16, 8, 16, 8, 16, 8, 16, 16, 16, 0, 0, 4, 8, 8, 16, 1, 2, 16, 1 << 20, 0]
+    for fn, args, at in ((k.qk_norm_rope, rope, (0, 1, 2, 3, 13, 15)), (k.kv_cache_write, cache, (8,)), (k.kv_cache_read, cache, (8,)),
+                         (k.paged_attention, att, (0, 9, 12, 19, 21)), (k.lora_add, lora, (0, 2, 4, 6, 7, 8, 17))):
+        for i in at:
+            with pytest.raises(ValueError, match="no memory"):
+                fn(*args[:i], 0, *args[i + 1:])
+    for rows, c in (([16, 0], c4), ([0, 16], c4), ([16, 16], [16, 0, 0, 0]), ([16, 16], [0, 16, 0, 0])):
+        with pytest.raises(ValueError, match="no memory"):
+            k.kv_cache_write(rows, st4, 2, c, *cache[4:])
+    with pytest.raises(ValueError, match="no memory"):
+        k.paged_attention(*att[:4], [16, 0, 0, 0], *att[5:])
