@@ -33,6 +33,8 @@ except ImportError:  # pragma: no cover
     torch = None
 
 if torch is not None:
+    import torch.autograd.forward_ad as _forward_ad
+
     _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3, torch.int8: 4}
     _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
     _INDEX = {torch.int32: 0, torch.int64: 1}
@@ -62,9 +64,17 @@ def _tensor(t, name, dim=None, dtypes=None, device=None, contiguous=False):
             raise ValueError(f"{name} must be contiguous")
     elif t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
+    _forward_only(t, name)
+    return t
+
+
+def _forward_only(t, name):
+    """Refuse a tensor whose gradient or tangent (forward mode) would be lost."""
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient; this operator is forward only (use torch.no_grad())")
-    return t
+    # a dual tensor does not require a gradient; outside of a dual level (-1) there are none
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name} has a tangent; this operator has no derivative (use forward_ad.unpack_dual(x).primal)")
 
 
 if torch is not None and hasattr(torch._C, "_cuda_getCurrentRawStream"):
@@ -214,6 +224,7 @@ def _cache(cache, device=None):
             raise ValueError(f"{name}: an 8-bit cache has scales")
         if not isinstance(s, torch.Tensor) or s.device != dev or s.dtype != torch.float32 or s.shape != k.shape[:3]:
             raise ValueError(f"{name} must be an fp32 tensor of {tuple(k.shape[:3])} on {dev}")
+        _forward_only(s, name)
     return k, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), st + ks.stride() + vs.stride()
 
 

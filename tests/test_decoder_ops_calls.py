@@ -96,3 +96,43 @@ def test_launchers_refuse_null_pointers(C):
             k.kv_cache_write(rows, st4, 2, c, *cache[4:])
     with pytest.raises(ValueError, match="no memory"):
         k.paged_attention(*att[:4], [16, 0, 0, 0], *att[5:])
+
+
+def test_gradients_of_both_modes_are_refused():
+    """Reverse mode by requires_grad, forward mode by a tangent (whose tensor does not require a gradient); the scales of an 8-bit
+    cache too."""
+    import torch.autograd.forward_ad as fw
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    f32, i32 = torch.float32, torch.int32
+    with FakeTensorMode():
+        q, k, n, inv = fake(4, 8, 64, dtype=f32), fake(4, 2, 64, dtype=f32), fake(4, dtype=i32), fake(32, dtype=f32)
+        x, y, A, B, ids = fake(6, 32, dtype=f32), fake(6, 48, dtype=f32), fake(3, 8, 32, dtype=f32), fake(3, 48, 8, dtype=f32), fake(6, dtype=i32)
+        qh, table = fake(4, 8, 64), fake(4, 3, dtype=i32)
+
+        def eight(f):
+            s = fake(5, 16, 2, dtype=f32)
+            return ops.KVCache(*(fake(5, 16, 2, 64, dtype=torch.int8) for _ in range(2)), s.clone(), f(s))
+
+        def calls(f):
+            return {
+                "q": lambda: ops.qk_norm_rope(f(q), k, None, None, n, inv),
+                "k": lambda: ops.qk_norm_rope(q, f(k), None, None, n, inv),
+                "q_weight": lambda: ops.qk_norm_rope(q, k, f(fake(64, dtype=f32)), None, n, inv),
+                "inv_freq": lambda: ops.qk_norm_rope(q, k, None, None, n, f(inv)),
+                "v": lambda: ops.kv_cache_write(ops.KVCache(fake(5, 16, 2, 64), fake(5, 16, 2, 64)), k, f(k.clone()), n),
+                "cache.v_scales": lambda: ops.kv_cache_read(eight(f), n),
+                " cache.v_scales": lambda: ops.paged_attention(qh, eight(f), table, n),
+                "y": lambda: ops.lora_add(f(y), x, A, B, ids),
+                "x": lambda: ops.lora_add(y, f(x), A, B, ids),
+                "B": lambda: ops.lora_add(y, x, A, f(B), ids),
+                "scales": lambda: ops.lora_add(y, x, A, B, ids, f(fake(3, dtype=f32))),
+            }
+
+        for name, call in calls(lambda t: t.clone().requires_grad_()).items():
+            with pytest.raises(RuntimeError, match=f"^{name.strip()} requires a gradient"):
+                call()
+        with fw.dual_level():
+            for name, call in calls(lambda t: fw.make_dual(t, torch.ones_like(t))).items():
+                with pytest.raises(RuntimeError, match=f"^{name.strip()} has a tangent"):
+                    call()
