@@ -64,12 +64,14 @@ def _tensor(t, name, dim=None, dtypes=None, device=None, contiguous=False):
             raise ValueError(f"{name} must be contiguous")
     elif t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    _forward_only(t, name)
+    _as_stored(t, name)
     return t
 
 
-def _forward_only(t, name):
-    """Refuse a tensor whose gradient or tangent (forward mode) would be lost."""
+def _as_stored(t, name):
+    """Refuse a tensor that is more than its memory says: a sign put off, a gradient or a tangent (forward mode)."""
+    if t.is_neg():
+        raise ValueError(f"{name} is a view whose sign is put off (the imaginary part of a conjugate); use {name}.resolve_neg()")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient; this operator is forward only (use torch.no_grad())")
     # a dual tensor does not require a gradient; outside of a dual level (-1) there are none
@@ -224,7 +226,7 @@ def _cache(cache, device=None):
             raise ValueError(f"{name}: an 8-bit cache has scales")
         if not isinstance(s, torch.Tensor) or s.device != dev or s.dtype != torch.float32 or s.shape != k.shape[:3]:
             raise ValueError(f"{name} must be an fp32 tensor of {tuple(k.shape[:3])} on {dev}")
-        _forward_only(s, name)
+        _as_stored(s, name)
     return k, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), st + ks.stride() + vs.stride()
 
 

@@ -136,3 +136,20 @@ def test_gradients_of_both_modes_are_refused():
             for name, call in calls(lambda t: fw.make_dual(t, torch.ones_like(t))).items():
                 with pytest.raises(RuntimeError, match=f"^{name.strip()} has a tangent"):
                     call()
+
+
+def test_views_whose_sign_is_put_off_are_refused():
+    """torch.conj(z).imag holds z's own numbers and a flag that says "negated", which a kernel does not see."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    f32, i32 = torch.float32, torch.int32
+    assert torch.ones(2, dtype=torch.complex64).conj().imag.is_neg()
+    with FakeTensorMode():
+        q = fake(4, 8, 1, dtype=torch.complex64).conj().imag  # a last dimension of one: any stride goes
+        assert q.is_neg()
+        with pytest.raises(ValueError, match="k is a view whose sign"):
+            ops.kv_cache_write(ops.KVCache(fake(5, 16, 8, 1), fake(5, 16, 8, 1)), q, fake(4, 8, 1, dtype=f32), fake(4, dtype=i32))
+        s = fake(5, 16, 2, dtype=torch.complex64).conj().imag
+        c = ops.KVCache(*(fake(5, 16, 2, 64, dtype=torch.int8) for _ in range(2)), fake(5, 16, 2, dtype=f32), s)
+        with pytest.raises(ValueError, match="cache.v_scales is a view whose sign"):
+            ops.kv_cache_read(c, fake(4, dtype=i32))
