@@ -177,6 +177,7 @@ template <class X, class C, int V> void launch(const KvCacheArgs& a, bool write,
   int lanes = 1, log2 = 0;
   while (lanes < 64 && lanes * V < a.dim) lanes *= 2, ++log2;
   const int64_t per = kThreads / lanes, blocks = (a.rows * a.heads.d + per - 1) / per;
+  need_blocks(blocks, kThreads, "kv_cache");
   const dim3 grid{unsigned(blocks)};
   if (write) launch_kernel(kv_cache_write_kernel<X, C, V>, grid, kThreads, 0, s, a, lanes, log2);
   else launch_kernel(kv_cache_read_kernel<X, C, V>, grid, kThreads, 0, s, a, lanes, log2);

@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -13,6 +14,11 @@ namespace sca::kern {
 // What a kernel reads or writes has an address: a tensor without memory (a fake one, as tracers use) has none.
 inline void need_memory(const void* p, const char* what) {
   if (!p) throw std::invalid_argument(std::string(what) + " has no memory");
+}
+
+// A launch holds fewer than 2^32 threads along x.  Asked before the first launch of a call, so that a call is refused whole.
+inline void need_blocks(int64_t blocks, int threads, const char* what) {
+  if (blocks > int64_t(0xffffffff) / threads) throw std::invalid_argument(std::string(what) + ": too large for one call");
 }
 
 template <class... P, class... A>

@@ -721,6 +721,7 @@ void lora_add(LoraArgs a, hipStream_t s) {
     throw std::invalid_argument("lora_add: sizes");
   if (a.rows <= 0) return;
   if (a.rows > 0x7fffff00) throw std::invalid_argument("lora_add: too many rows for one call");
+  need_blocks((a.rows + 31) / 32, 64 * kDownWaves<32>, "lora_add");  // few rows have far fewer, as "up" has
   need_memory(a.x, "lora_add: x");
   need_memory(a.y, "lora_add: y");
   need_memory(a.out, "lora_add: out");

@@ -554,10 +554,14 @@ template <class T, int DP> __global__ __launch_bounds__(kThreads) void paged_att
     a.lse[out_row] = sum > 0.f || sum != sum ? (top + log2f(sum)) / kLog2e : -INFINITY;
 }
 
+// A request of one step at most is never split.
+bool joins(const PagedAttentionArgs& a) {
+  return (a.window > 0 && a.window < a.max_tokens ? a.window : a.max_tokens) > kStep;
+}
+
 template <class T, class C, int DP> void launch(const PagedAttentionArgs& a, hipStream_t s) {
   launch_kernel(paged_attention_kernel<T, C, DP>, dim3(unsigned(a.grid)), kThreads, 0, s, a);
-  // a request of one step at most is never split
-  if ((a.window > 0 && a.window < a.max_tokens ? a.window : a.max_tokens) > kStep)
+  if (joins(a))
     launch_kernel(paged_attention_join<T, DP>, dim3(unsigned(a.batch * a.q_heads)), kThreads, 0, s, a, a.grid);
 }
 
@@ -605,6 +609,7 @@ int64_t paged_attention_plan(PagedAttentionArgs& a) {
   a.row_blocks = (a.group + 15) / 16;
   a.partial_rows = a.group < 16 ? a.group : 16;
   if (int64_t(a.batch) * a.q_heads > 0x7fffffff) throw std::invalid_argument("paged_attention: too large for one call");
+  if (joins(a)) need_blocks(int64_t(a.batch) * a.q_heads, kThreads, "paged_attention");
   a.grid = grid_of(a.batch, a.kv_heads, a.row_blocks, a.dim, width == 1, a.max_tokens, a.window);
   return workspace_of(a.grid, a.partial_rows, a.dim);
 }

@@ -146,6 +146,7 @@ template <class T, int V> void launch(const QkNormRopeArgs& a, hipStream_t s) {
   // whole tokens for each workgroup: one while they are few, so that each has a CU of its own
   int64_t tb = a.tokens / 1024;
   tb = tb < 1 ? 1 : tb > 4 ? 4 : tb;
+  need_blocks((a.tokens + tb - 1) / tb, kThreads, "qk_norm_rope");
   const unsigned grid = unsigned((a.tokens + tb - 1) / tb);
   const FastDiv by_half{uint32_t(half)}, by_heads{uint32_t(a.heads[0] + a.heads[1])};
   const size_t lds = size_t(2 * a.dim + tb * a.dim) * sizeof(float);
@@ -174,7 +175,6 @@ void qk_norm_rope(const QkNormRopeArgs& a, hipStream_t s) {
   if (a.n_freq < 0 || 2 * a.n_freq > a.dim) throw std::invalid_argument("qk_norm_rope: 2 * n_freq <= dim");
   if (a.heads[0] < 0 || a.heads[1] < 0) throw std::invalid_argument("qk_norm_rope: heads");
   if (a.tokens <= 0 || a.heads[0] + a.heads[1] == 0) return;
-  if (a.tokens > int64_t(1) << 32) throw std::invalid_argument("qk_norm_rope: too many tokens");
   for (int i = 0; i < 2; ++i) {
     if (!a.heads[i]) continue;
     need_memory(a.x[i], "qk_norm_rope: an input");

@@ -153,3 +153,18 @@ def test_views_whose_sign_is_put_off_are_refused():
         c = ops.KVCache(*(fake(5, 16, 2, 64, dtype=torch.int8) for _ in range(2)), fake(5, 16, 2, dtype=f32), s)
         with pytest.raises(ValueError, match="cache.v_scales is a view whose sign"):
             ops.kv_cache_read(c, fake(4, dtype=i32))
+
+
+def test_calls_too_large_for_a_launch_are_refused_whole(C):
+    """A launch has fewer than 2^32 threads along x: what would need more is refused before the first launch."""
+    k = C.kernels
+    st4, st12, c4 = [64] * 4, [64] * 12, [16] * 4
+    with pytest.raises(ValueError, match="too large"):  # 2^26 tokens, 4 a workgroup of 256 threads
+        k.qk_norm_rope(16, 16, 16, 16, 0, 0, False, [1] * 8, 1 << 26, 2, 2, 8, 2, 16, 0, 16, 0, 2, False, 1e-6, 0)
+    for fn in (k.kv_cache_write, k.kv_cache_read):  # dim 512: a wave for each of 2^26 heads
+        with pytest.raises(ValueError, match="too large"):
+            fn([16, 16], st4, 2, c4, st12, 2, 2, 16, 16, 0, 1 << 23, 8, 512, 0)
+    with pytest.raises(ValueError, match="too large"):  # 2^18 requests of 64 heads: a workgroup each to join their parts
+        k.paged_attention(16, 64, 64, 2, c4, st12, 2, 5, 16, 16, 16, 16, 16, 1 << 18, 8, 8, 64, 0, 1.0, 16, 0, 16, 1 << 40, 0)
+    with pytest.raises(ValueError, match="too large"):  # 2^28 rows, 32 a workgroup of 512 threads
+        k.lora_add(16, 8, 16, 8, 16, 8, 16, 16, 16, 0, 0, 1 << 28, 8, 8, 16, 1, 2, 16, 1 << 50, 0)
