@@ -19,8 +19,8 @@
 // - Only V has to be turned: through LDS (private to the wave, no barrier) and the
 //   transposing LDS read.  Its rows are 32 bytes longer than the data, which makes
 //   the 16-byte writes and the 8-byte transposed reads free of bank conflicts.
-// - The maximum is taken over lanes and the sums rescaled only when some score
-//   exceeds the reference by more than 2^kSlack, which after the first tile is rare.
+// - The maximum is taken over lanes and the sums rescaled only when some weight
+//   exceeds 2^kSlack, which after the first tile is rare.
 // - 8-bit caches are widened to the 16-bit operand, exactly; K's scale multiplies
 //   the score and V's the weight, so no element is multiplied by its scale.
 //
@@ -28,7 +28,9 @@
 // go into it as the sum of two 16-bit numbers (high part and remainder), since one
 // rounding of each to bf16 would cost as much as the output's own; the second
 // instruction hides behind the loads.  With an fp16 V the weights are held times
-// 2^12, so that the small ones of a long context stay clear of fp16's subnormals.
+// 2^12, so that the small ones of a long context stay clear of fp16's subnormals
+// (2^(12 + kSlack) is in its range).  The 12 is added to a score's distance from
+// the reference, never to the reference: of scores from 2^25 on fp32 would round it.
 //
 // Work is split evenly whatever the lengths: the 128-token steps of all (request,
 // key head) pairs form one sequence, of which every workgroup takes an equal run,
@@ -129,7 +131,7 @@ template <class T, class C, int DP> struct Shape {
   static constexpr int kRun = 16 / sizeof(C);         // elements of a lane's 16 bytes
   static constexpr int kRuns = DP / (4 * kRun);       // 16-byte pieces of a row for each lane
   static constexpr int kRow = DP + 16;                // elements of a row of V in LDS
-  static constexpr float kRaise = std::is_same_v<V, f16> ? 12.f : 0.f;
+  static constexpr float kRaise = std::is_same_v<V, f16> ? 12.f : 0.f, kLower = std::is_same_v<V, f16> ? 0x1p-12f : 1.f;
   static constexpr float kSlack = std::is_same_v<V, f16> ? 3.f : 8.f;
   static constexpr int kWaveLds = kTile * kRow * 2;   // bytes; also holds 16 x DP floats at the end
   static constexpr int kOutRow = DP + 4;
@@ -361,10 +363,10 @@ __global__ __launch_bounds__(kThreads, resident(DP, kQuantised<C>)) void paged_a
         float top = sc[0][0];
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, fmaxf(sc[0][r], sc[1][r]));
-        if (__any(top > m + S::kRaise + S::kSlack)) {
+        if (__any(top - m > S::kSlack)) {
           top = fmaxf(top, __shfl_xor(top, 16));
           top = fmaxf(top, __shfl_xor(top, 32));
-          const float m_new = fmaxf(m, top - S::kRaise);
+          const float m_new = fmaxf(m, top);
           const float alpha = m_new > -INFINITY ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
           m = m_new;
           l *= alpha;
@@ -379,7 +381,7 @@ __global__ __launch_bounds__(kThreads, resident(DP, kQuantised<C>)) void paged_a
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float p = __builtin_amdgcn_exp2f(sc[h][r] - ref);
+            float p = __builtin_amdgcn_exp2f(S::kRaise > 0.f ? (sc[h][r] - ref) + S::kRaise : sc[h][r] - ref);
             l += p;
             if constexpr (S::kQ8) {
               // a masked token's scale may be anything; its weight stays 0
@@ -415,7 +417,7 @@ __global__ __launch_bounds__(kThreads, resident(DP, kQuantised<C>)) void paged_a
     const float ref = top > -INFINITY ? top : 0.f;
     float* const ol = reinterpret_cast<float*>(smem + wave * S::kWaveLds);
     {
-      const float f = __builtin_amdgcn_exp2f(m - ref);
+      const float f = __builtin_amdgcn_exp2f(m - ref) * S::kLower;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         f32x4 x;
@@ -425,7 +427,7 @@ __global__ __launch_bounds__(kThreads, resident(DP, kQuantised<C>)) void paged_a
       }
     }
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += wave_l[w][n16] * __builtin_amdgcn_exp2f(wave_m[w][n16] - ref);
+    for (int w = 0; w < kWaves; ++w) sum += wave_l[w][n16] * (__builtin_amdgcn_exp2f(wave_m[w][n16] - ref) * S::kLower);
     __syncthreads();
     const bool whole = count == uint32_t(sp.steps);
     const int64_t out_row = int64_t(b) * a.q_heads + head * a.group + row0;

@@ -168,3 +168,46 @@ def test_calls_too_large_for_a_launch_are_refused_whole(C):
         k.paged_attention(16, 64, 64, 2, c4, st12, 2, 5, 16, 16, 16, 16, 16, 1 << 18, 8, 8, 64, 0, 1.0, 16, 0, 16, 1 << 40, 0)
     with pytest.raises(ValueError, match="too large"):  # 2^28 rows, 32 a workgroup of 512 threads
         k.lora_add(16, 8, 16, 8, 16, 8, 16, 16, 16, 0, 0, 1 << 28, 8, 8, 16, 1, 2, 16, 1 << 50, 0)
+
+
+# --------------------------------------------------------- values at the ends
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+CACHE = {"same": None, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float32):
+    return torch.randn(shape, generator=g).to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_paged_attention_scores_as_large_as_the_types_give(dtype, cache):
+    """Scores of 2^20 to 2^29, a few ulps apart, where fp32 has no room for the distance that weights are kept at.
+
+    All tokens hold the same value, so whatever the weights are, the output is that value: weights that are split, w (1 +- 2^-16), and
+    n + 64 fp32 roundings of the sums, and one rounding to the type."""
+    g, dt, n, D = gen(3), DT[dtype], 700, 64
+    for power in range(20, 30):
+        c = ops.kv_cache(-(-n // 16), 16, 1, D, dtype=CACHE[cache] or dt)
+        k = torch.zeros((n, 1, D))
+        k[:, 0, 0] = 2.0 ** (power - 14)
+        k[:, 0, 1] = torch.randint(0, 200, (n,), generator=g) if cache == "same" else 0
+        k[:, 0, 0] *= 1 if cache == "same" else 1 + torch.randint(0, 2, (n,), generator=g) / 8  # steps that e4m3 has
+        # 8 bits hold powers of two exactly, under whatever scale
+        value = torch.tensor([1.0, -2.0, 0.5, 0.25, 0.0, 1.0, -1.0, -0.125]).repeat(D // 8) if cache != "same" else randn(g, D, dtype=dt).float()
+        v = value.expand(n, 1, D)
+        ops.kv_cache_write(c, k.to(dt).cuda(), v.to(dt).cuda(), torch.arange(n).cuda())
+        q = torch.zeros((1, 2, D), dtype=dt)
+        q[..., 0], q[..., 1] = 2.0 ** 14, 1
+        table, lens = torch.arange(-(-n // 16)).int()[None].cuda(), torch.tensor([n]).int().cuda()
+        out, lse = ops.paged_attention(q.cuda(), c, table, lens, scale=1.0, return_lse=True)
+        rel = torch.finfo(dt).eps / 2 + 2.0 ** -16 + (n + 64) * 2.0 ** -24
+        assert bool(((out.cpu().double() - value.double()).abs() <= rel * value.abs().double()).all()), f"2^{power}: {out[0, 0, :4]}"
+        s = k[:, 0, 0].double() * 2.0 ** 14 + k[:, 0, 1].double()
+        # the products' sum, its product with log2(e), and the way back: a few roundings of the score
+        assert bool(((lse.cpu().double() - torch.logsumexp(s, 0)).abs() <= 4 * 2.0 ** -24 * float(s.max()) + 1e-4).all())
