@@ -306,7 +306,11 @@ __global__ __launch_bounds__(kThreads, resident(DP, kQuantised<C>)) void paged_a
       if constexpr (S::kQ8) {
         if (g4 == 0) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) ksc[h * 16 + n16] = kscale[h] * to_log2, vsc[h * 16 + n16] = vscale[h];
+          for (int h = 0; h < 2; ++h) {
+            ksc[h * 16 + n16] = kscale[h] * to_log2;
+            // a token that does not exist has any scale: its weight is 0 and has to stay so
+            vsc[h * 16 + n16] = ok[h] >> n16 & 1 ? vscale[h] : 0.f;
+          }
         }
       }
       // V of this tile to LDS; rows that do not exist as zeros (0 * NaN would not be 0)
@@ -383,10 +387,7 @@ __global__ __launch_bounds__(kThreads, resident(DP, kQuantised<C>)) void paged_a
           for (int r = 0; r < 4; ++r) {
             float p = __builtin_amdgcn_exp2f(S::kRaise > 0.f ? (sc[h][r] - ref) + S::kRaise : sc[h][r] - ref);
             l += p;
-            if constexpr (S::kQ8) {
-              // a masked token's scale may be anything; its weight stays 0
-              p = p > 0.f || p != p ? p * vsc4[h][r] : 0.f;
-            }
+            if constexpr (S::kQ8) p *= vsc4[h][r];  // NaN under a scale of NaN, also where the weight is 0 in fp32
             hi[h * 4 + r] = V(p);
             lo[h * 4 + r] = V(p - float(hi[h * 4 + r]));
           }

@@ -311,8 +311,13 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
     of 8, of 16 with 8 bits), starting at one.  A length beyond the table counts
     as the table's end, a negative one as 0; tokens on a page outside the cache
     are left out, and what the cache holds where nothing is seen (anything, NaN
-    too) does not matter.  A request that sees nothing gets zeros.  A value that
-    is seen and is infinite or NaN makes its dimension NaN.
+    too) does not matter.  A request that sees nothing, or nothing but scores of
+    -inf, gets zeros.  Where a value that is seen is NaN, so is its dimension;
+    where one is infinite its dimension is infinite or NaN, never finite (a
+    weight enters as the sum of two 16-bit numbers, of which one can be 0 or
+    negative).  In 8 bits the head's scale is NaN then, and so are all of its
+    dimensions.  Sums are fp32 and divided by the softmax's total at the end, so
+    values beyond about 10^30 can overflow.
 
     Returns [B, Hq, D] in q's type (``out`` if given: contiguous, not
     overlapping q), with ``return_lse`` also the natural logsumexp of its scores

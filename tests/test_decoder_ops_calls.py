@@ -211,3 +211,35 @@ def test_paged_attention_scores_as_large_as_the_types_give(dtype, cache):
         s = k[:, 0, 0].double() * 2.0 ** 14 + k[:, 0, 1].double()
         # the products' sum, its product with log2(e), and the way back: a few roundings of the score
         assert bool(((lse.cpu().double() - torch.logsumexp(s, 0)).abs() <= 4 * 2.0 ** -24 * float(s.max()) + 1e-4).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["same", "e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_paged_attention_values_that_are_not_finite(dtype, cache):
+    """One token's value of a request is infinite or NaN.  Seen, the dimension it is in (with 8 bits, which keep one scale for the
+    head: the head) is not finite, however small the token's weight; outside of the window it does not matter."""
+    g, dt, n, H, D = gen(4), DT[dtype], 300, 2, 64
+    for bad in (math.inf, -math.inf, math.nan):
+        for depth in (0.0, 2.0, 400.0):  # the token's score below the others: its weight is ordinary, small, or 0 in fp32
+            c = ops.kv_cache(-(-n // 16), 16, H, D, dtype=CACHE[cache] or dt)
+            k, v = 0.1 * randn(g, n, H, D), randn(g, n, H, D)
+            k[..., 0] = 1
+            k[100, 1, 0] = 1 - depth / 8
+            v[100, 1, 7] = bad
+            q = 0.1 * randn(g, 1, 2 * H, D)
+            q[..., 0] = 8
+            ops.kv_cache_write(c, k.to(dt).cuda(), v.to(dt).cuda(), torch.arange(n).cuda())
+            table, lens = torch.arange(-(-n // 16)).int()[None].cuda(), torch.tensor([n]).int().cuda()
+            out, lse = (x.cpu() for x in ops.paged_attention(q.to(dt).cuda(), c, table, lens, scale=1.0, return_lse=True))
+            assert torch.isfinite(out[:, :2]).all() and torch.isfinite(lse).all()
+            hit = torch.zeros(D, dtype=torch.bool)
+            hit[7] = True
+            if cache != "same":
+                hit[:] = True
+            assert not torch.isfinite(out[:, 2:, hit]).any(), (bad, depth, out[0, 2, :8])
+            assert torch.isfinite(out[:, 2:, ~hit]).all()
+            if cache != "same" or math.isnan(bad):
+                assert out[:, 2:, hit].isnan().all()
+            out = ops.paged_attention(q.to(dt).cuda(), c, table, lens, scale=1.0, window=n - 101)
+            assert torch.isfinite(out).all()
