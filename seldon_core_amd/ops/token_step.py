@@ -375,8 +375,11 @@ def lora_add(y, x, A, B, adapters, scales=None, out=None):
     negative or behind the last keeps y.  Rows may come in any order; many rows
     are fastest where those of one adapter lie together.
 
-    Sums are fp32, with one rounding at the end; an infinite weight of B gives
-    NaN.  Returns a new tensor, or ``out``, which may be ``y`` itself (other overlaps are not allowed).
+    Sums are fp32, with one rounding at the end.  Where a weight of B is infinite
+    the result is: with fp32 tensors the infinity (or, next to a 0, the NaN) that
+    the formula has; with 16-bit ones infinite or NaN, since ``A x`` enters the
+    second product as the sum of two 16-bit numbers.  Returns a new tensor, or
+    ``out``, which may be ``y`` itself (other overlaps are not allowed).
     """
     global _lora_workspace
     _tensor(y, "y", 2, _FLOATS)

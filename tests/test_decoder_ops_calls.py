@@ -243,3 +243,32 @@ def test_paged_attention_values_that_are_not_finite(dtype, cache):
                 assert out[:, 2:, hit].isnan().all()
             out = ops.paged_attention(q.to(dt).cuda(), c, table, lens, scale=1.0, window=n - 101)
             assert torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 700])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_lora_add_weights_that_are_not_finite(dtype, T):
+    """An infinite or NaN weight of B reaches its own column of its own adapter's rows, and one of A all columns of them."""
+    g, dt = gen(5), DT[dtype]
+    K, M, r, N = 96, 130, 12, 3
+    x, y = randn(g, T, K, dtype=dt), randn(g, T, M, dtype=dt)
+    A, B = (randn(g, N, r, K) * 0.1).to(dt), randn(g, N, M, r, dtype=dt)
+    ids = (torch.arange(T) * 7 % (N + 1)).int()  # N: none
+    hit = ids == 1
+    for bad in (math.inf, -math.inf, math.nan):
+        b = B.clone()
+        b[1, 70, 11] = bad
+        got = ops.lora_add(y.cuda(), x.cuda(), A.cuda(), b.cuda(), ids.cuda()).cpu()
+        assert not torch.isfinite(got[hit][:, 70]).any()
+        if dtype == "fp32" and not math.isnan(bad):  # h in one piece: the formula's own infinity
+            sign = torch.sign(x[hit].double() @ A[1, 11].double())
+            assert torch.equal(got[hit][:, 70].double(), sign * bad)
+        a = A.clone()
+        a[1, 11, 95] = bad
+        some = ops.lora_add(y.cuda(), x.cuda(), a.cuda(), B.cuda(), ids.cuda()).cpu()
+        assert not torch.isfinite(some[hit]).any()
+        for o, keep in ((got, torch.ones(M, dtype=torch.bool)), (some, torch.ones(M, dtype=torch.bool))):
+            assert torch.isfinite(o[~hit]).all() and torch.equal(o[ids == N], y[ids == N])
+        cols = torch.arange(M) != 70
+        assert torch.isfinite(got[:, cols]).all()
