@@ -13,7 +13,9 @@ null stream (see :class:`~seldon_core_amd.models.cnn.CompiledCnn`).
 The module must be row-wise (row i of the output depends only on row i of the
 input) -- the contract batched serving already assumes -- and
 capture-safe (no host synchronisation or data-dependent control flow inside
-``forward``).  A module whose capture fails is served eagerly from then on,
+``forward``).  It must keep nothing between calls: before the capture it runs on
+rows of zeros, and a batch is padded with them.  A key-value cache is kept, so
+``ops.kv_cache_write`` refuses such a run.  A module whose capture fails is served eagerly from then on,
 with the reason kept in ``graph_error``.
 """
 from __future__ import annotations
@@ -50,15 +52,18 @@ class GraphedModule:
         return min(b, self.max_batch)
 
     def _capture(self, key: Tuple) -> Optional[tuple]:
+        from ..ops.token_step import no_cache_writes
+
         bs, row_shape = key[0], key[1:]
         x = torch.zeros((bs,) + row_shape, device=self.device, dtype=self.in_dtype)
-        with torch.no_grad(), torch.cuda.stream(self.stream):
-            for _ in range(2):  # library algorithm choice / workspaces before capture
-                self.module(x)
-        self.stream.synchronize()
-        g = torch.cuda.CUDAGraph()
-        with torch.no_grad(), torch.cuda.graph(g, stream=self.stream):
-            y = self.module(x)
+        with no_cache_writes("rows of zeros, and padding later, are no request's (GraphedModule)"):
+            with torch.no_grad(), torch.cuda.stream(self.stream):
+                for _ in range(2):  # library algorithm choice / workspaces before capture
+                    self.module(x)
+            self.stream.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.no_grad(), torch.cuda.graph(g, stream=self.stream):
+                y = self.module(x)
         return g, x, y
 
     def _graph_for(self, key: Tuple) -> Optional[tuple]:

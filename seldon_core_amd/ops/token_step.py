@@ -1,8 +1,7 @@
 """Operators of one step of a served token model.
 
-A decoder's attention block between its projections, as a GPU component or a
-captured module (:class:`~seldon_core_amd.models.graphed.GraphedModule`) calls
-it::
+A decoder's attention block between its projections, as a GPU component calls
+it, eagerly or through a graph that it captures::
 
     qkv = ops.lora_add(F.linear(x, w_qkv), x, A, B, tenant)     # adapters of many tenants
     q, k, v = qkv.view(T, -1, D).split((Hq, Hk, Hk), 1)
@@ -18,11 +17,19 @@ see (shapes, types, strides, devices, tensors without memory, as tracers use
 them) is checked and refused with ``ValueError`` / ``TypeError``; indices that point outside a cache or a table
 are left out by the kernels as each op says.  The ops are forward only.
 
+A captured step pads its batch with rows whose slot is -1 (nothing is written)
+and whose length is 0.  :class:`~seldon_core_amd.models.graphed.GraphedModule`
+pads with zeros and runs a module on zeros before it captures it, which is right
+for modules that keep nothing; in it ``kv_cache_write`` raises, and a module
+that writes a cache is served eagerly.
+
 Kernel sources: csrc/kernels/{rope,kv_cache,paged_attention,lora}.hip.
 """
 from __future__ import annotations
 
+import contextlib
 import functools
+import threading
 from typing import NamedTuple, Optional, Tuple
 
 from .._native import native
@@ -230,6 +237,19 @@ def _cache(cache, device=None):
     return k, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), st + ks.stride() + vs.stride()
 
 
+_rehearsal = threading.local()
+
+
+@contextlib.contextmanager
+def no_cache_writes(why: str):
+    """In this thread :func:`kv_cache_write` raises: for callers that run a module on rows that are no request's."""
+    before, _rehearsal.why = getattr(_rehearsal, "why", None), why
+    try:
+        yield
+    finally:
+        _rehearsal.why = before
+
+
 def _slots(slots, device):
     _tensor(slots, "slots", 1, _INDEX, device, contiguous=True)
     return slots.shape[0]
@@ -248,6 +268,8 @@ def kv_cache_write(cache: KVCache, k, v, slots) -> KVCache:
     the cache is left out (padding).  Slots must not name the same place twice:
     which row's values it would hold is not defined.
     """
+    if getattr(_rehearsal, "why", None):
+        raise RuntimeError(f"the cache is not written: {_rehearsal.why}")
     c, ptrs, cst = _cache(cache)
     dev = c.device
     pages, page, heads, dim = c.shape

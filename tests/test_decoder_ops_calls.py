@@ -272,3 +272,60 @@ def test_lora_add_weights_that_are_not_finite(dtype, T):
             assert torch.isfinite(o[~hit]).all() and torch.equal(o[ids == N], y[ids == N])
         cols = torch.arange(M) != 70
         assert torch.isfinite(got[:, cols]).all()
+
+
+# ------------------------------------------------------------- captured calls
+class CacheStep(torch.nn.Module):
+    """Rows of [slot, values]: writes each row's key and value at its slot, and gives back what the cache then holds there."""
+
+    def __init__(self, cache):
+        super().__init__()
+        self.cache = cache
+
+    def forward(self, x):
+        slots, k = x[:, 0].long(), x[:, 1:].reshape(len(x), *self.cache.k.shape[2:])
+        ops.kv_cache_write(self.cache, k, 2 * k, slots)
+        k, v = ops.kv_cache_read(self.cache, slots)
+        return k.flatten(1) + v.flatten(1)
+
+
+@pytest.mark.gpu
+def test_graphed_module_leaves_a_cache_to_its_rows():
+    """GraphedModule runs a module on zeros before it captures it, and pads batches with zeros: rows that would be written at slot 0
+    of a live request.  A module that writes a cache is served eagerly, each row once."""
+    from seldon_core_amd.models.graphed import GraphedModule
+
+    cache = ops.kv_cache(4, 4, 2, 8, dtype=torch.float32)
+    live = torch.full((1, 2, 8), 5.0, device="cuda")
+    ops.kv_cache_write(cache, live, live, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    m = GraphedModule(CacheStep(cache), max_batch=8)
+    g = gen(6)
+    for n in (3, 11, 5):  # buckets of 4, 8 + 4 and 8
+        x = randn(g, n, 17)
+        x[:, 0] = 1 + torch.randperm(15, generator=g)[:n]
+        out = m(x.numpy())
+        assert torch.equal(torch.from_numpy(out), 3 * x[:, 1:])
+        assert torch.equal(cache.k[0, 0], live[0]) and torch.equal(cache.v[0, 0], live[0])
+    assert "cache" in m.graph_error and m.replays == 0 and m.eager_calls == 4
+
+    class Reader(torch.nn.Module):  # what only reads is captured
+        def forward(self, x):
+            k, _ = ops.kv_cache_read(cache, x[:, 0].long())
+            return k.flatten(1)
+
+    r = GraphedModule(Reader(), max_batch=8)
+    x = torch.zeros(3, 1)
+    assert torch.equal(torch.from_numpy(r(x.numpy())), live.flatten(1).cpu().expand(3, 16)) and r.graph_error is None and r.replays == 1
+
+
+def test_a_cache_is_not_written_in_a_rehearsal():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        cache, k = ops.KVCache(fake(5, 16, 2, 64), fake(5, 16, 2, 64)), fake(0, 2, 64)
+        write = lambda: ops.kv_cache_write(cache, k, k, fake(0, dtype=torch.int32))  # noqa: E731
+        assert write() is cache
+        with ops.token_step.no_cache_writes("rows of zeros"):
+            with pytest.raises(RuntimeError, match="rows of zeros"):
+                write()
+        assert write() is cache
