@@ -477,6 +477,8 @@ class Step(torch.nn.Module):
         self.cache = ops.kv_cache(pages, page, H, D, dtype=cache)
 
     def forward(self, x, tenant, positions, table):
+        if not torch.cuda.is_current_stream_capturing():  # inputs and cache are made on the default stream
+            torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
         Hq, H, D = self.Hq, self.H, self.D
         y = x @ self.w.T
         y = ops.lora_add(y, x, self.A, self.B, tenant, out=y).view(len(x), -1, D)

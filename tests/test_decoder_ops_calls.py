@@ -329,3 +329,33 @@ def test_a_cache_is_not_written_in_a_rehearsal():
             with pytest.raises(RuntimeError, match="rows of zeros"):
                 write()
         assert write() is cache
+
+
+@pytest.mark.gpu
+def test_a_step_on_a_side_stream_waits_for_its_inputs():
+    """The block of test_decoder_ops on a stream of its own, while the default stream has yet to make its inputs: it orders itself
+    behind them.  (Either way every index is a valid one: the inputs hold an earlier step's.)"""
+    from test_decoder_ops import Step, step_inputs
+
+    T, page, W, Hq, H, D, tenants = 5, 16, 4, 8, 2, 64, 3
+    g = gen(21)
+    m = Step(256, Hq, H, D, tenants, T * W, page, torch.bfloat16, g)
+    table = torch.randperm(T * W, generator=g).int().view(T, W).cuda()
+    old, new = (step_inputs(g, T, tenants, W, page, 3 + 20 * i) for i in range(2))
+    with torch.no_grad():
+        m(*old, table)
+        want = m(*new, table).clone()
+        for c in m.cache[:2]:
+            c.zero_()
+        m(*old, table)
+        sx, st, sp = (t.clone() for t in old)
+        side, a = torch.cuda.Stream(), torch.randn(8192, 8192, device="cuda")
+        torch.cuda.synchronize()
+        for _ in range(5):  # tens of milliseconds in front of the inputs
+            a @ a
+        for s, n in zip((sx, st, sp), new):
+            s.copy_(n)
+        with torch.cuda.stream(side):
+            got = m(sx, st, sp, table)
+        torch.cuda.synchronize()
+    assert torch.equal(got, want)
