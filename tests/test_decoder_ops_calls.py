@@ -359,3 +359,71 @@ def test_a_step_on_a_side_stream_waits_for_its_inputs():
             got = m(sx, st, sp, table)
         torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------- adapters: the larger forms
+def lora_check(got, y, x, A, B, ids, scales):
+    """As test_decoder_ops has it: two sums in fp32 ((K + r + 8) 2^-24 of the sum of magnitudes), h in two 16-bit parts (2^-16 of it
+    in bf16, 2^-24 of the row's largest h in fp16, whose remainder may be subnormal), one rounding to the type."""
+    from test_decoder_ops import close
+
+    (N, r, K), dt = A.shape, x.dtype
+    want, mag = ops.token_step.lora_add_ref(y, x, A, B, ids, scales)
+    atol = (K + r + 8) * 2.0 ** -24 * mag + (2.0 ** -16 * mag if dt == torch.bfloat16 else 0)
+    if dt == torch.float16:
+        for a in range(N):
+            rows = ids == a
+            h = (x[rows].double() @ A[a].double().T).abs().amax(-1, keepdim=True) * (1.0 if scales is None else abs(scales[a].double()))
+            atol[rows] += 2.0 ** -23 * h * B[a].double().abs().sum(-1)
+    close(got, want, dt, atol + 2.0 ** -24 * want.abs())
+    none = (ids < 0) | (ids >= N)
+    assert torch.equal(got.cpu()[none], y[none])
+
+
+LORA = [  # rows, inner, outer, rank, adapters, mixed: many rows of uneven ranks, one and several column tiles of a workgroup, ends inside
+    (1500, 200, 1100, 12, 6, True), (1500, 72, 3000, 13, 6, True), (700, 130, 330, 27, 5, True), (1300, 130, 3300, 27, 4, False),
+    (300, 136, 1503, 99, 4, True), (900, 136, 5000, 99, 3, True), (2000, 96, 2100, 9, 3, False), (400, 200, 1000, 77, 3, True),
+    (330, 96, 640, 100, 5, True), (400, 160, 700, 128, 3, False), (300, 64, 4000, 50, 2, True),
+    # four rows of a workgroup, several column tiles
+    (512, 100, 1100, 8, 6, True), (120, 64, 5000, 64, 4, True), (130, 72, 6000, 27, 3, True), (64, 64, 9000, 101, 2, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", LORA, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("dtype", list(DT))
+def test_lora_add_larger_forms(case, dtype):
+    T, K, M, r, N, mixed = case
+    g, dt = gen(sum(case)), DT[dtype]
+    x, y = randn(g, T, K, dtype=dt), randn(g, T, M, dtype=dt)
+    A, B, scales = (randn(g, N, r, K) * K ** -0.5).to(dt), (randn(g, N, M, r) * r ** -0.5).to(dt), randn(g, N)
+    ids = torch.randint(-1, N + 1, (T,), generator=g) if mixed else torch.arange(T) * N // T
+    ids[-1] = N - 1  # the last adapter's last run, with nothing behind it
+    got = ops.lora_add(y.cuda(), x.cuda(), A.cuda(), B.cuda(), ids.cuda(), scales.cuda())
+    lora_check(got, y, x, A, B, ids, scales)
+
+
+@pytest.mark.gpu
+def test_lora_add_sorted_rows_in_a_captured_graph():
+    """A large mixed batch, sorted by a launch of its own: replays with other rows and adapters, with eager calls in between, give
+    what eager calls give; one of the replays has its rows in runs, which leaves the sort out."""
+    g = gen(7)
+    T, K, M, r, N = 900, 128, 192, 16, 40
+    A, B = ((randn(g, *s) * 0.1).bfloat16() for s in ((N, r, K), (N, M, r)))
+    steps = [(randn(g, T, K, dtype=torch.bfloat16), randn(g, T, M, dtype=torch.bfloat16), torch.randint(-1, N, (T,), generator=g)) for _ in range(4)]
+    steps[2][2].copy_(torch.sort(steps[2][2]).values // 4)
+    Ad, Bd = A.cuda(), B.cuda()
+    static = [t.cuda() for t in steps[0]]
+    graph = torch.cuda.CUDAGraph()
+    ops.lora_add(static[1], static[0], Ad, Bd, static[2])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = ops.lora_add(static[1], static[0], Ad, Bd, static[2])
+    for x, y, ids in steps:
+        for s, t in zip(static, (x, y, ids)):
+            s.copy_(t)
+        graph.replay()
+        eager = ops.lora_add(static[1], static[0], Ad, Bd, static[2])
+        other = ops.lora_add(static[1], static[0], Ad, Bd, (static[2] + 1) % N)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and not torch.equal(out, other)
+        lora_check(out, y, x, A, B, ids, None)
