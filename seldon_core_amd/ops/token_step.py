@@ -45,6 +45,8 @@ if torch is not None:
     _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3, torch.int8: 4}
     _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
     _INDEX = {torch.int32: 0, torch.int64: 1}
+    _NEGATED = (torch.float32, torch.float16)  # types that views of complex numbers have
+    _Tensor = torch.Tensor
 
 _kernels = None
 
@@ -56,22 +58,26 @@ def _k():
     return _kernels
 
 
-def _tensor(t, name, dim=None, dtypes=None, device=None, contiguous=False):
-    """Refuse what the kernels do not take; ``contiguous``: every stride, else only the last."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+# A call's checks are most of its host time, which bounds the small ones (about 0.1 us for each question asked of a tensor):
+# nothing is asked twice, and rare properties only where the type can have them.
+def _tensor(t, name, dim, dtypes, device=None, contiguous=False):
+    """Refuse what the kernels do not take; ``contiguous``: every stride, else only the last.  ``device``: a GPU."""
+    if not isinstance(t, _Tensor) or (not t.is_cuda if device is None else t.device != device):
+        if isinstance(t, _Tensor) and t.is_cuda:
+            raise ValueError(f"{name} is on {t.device}, not {device}")
         raise ValueError(f"{name} must be a GPU tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not {device}")
-    if dim is not None and t.dim() != dim:
+    if t.dim() != dim:
         raise ValueError(f"{name} must have {dim} dimensions, got {tuple(t.shape)}")
-    if dtypes is not None and t.dtype not in dtypes:
-        raise TypeError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
+    dtype = t.dtype
+    if dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {[str(d) for d in dtypes]}, got {dtype}")
     if contiguous:
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-    elif t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
+    elif t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    _as_stored(t, name)
+    if t.requires_grad or _forward_ad._current_level >= 0 or dtype in _NEGATED and t.is_neg():
+        _as_stored(t, name)
     return t
 
 
@@ -86,17 +92,21 @@ def _as_stored(t, name):
         raise RuntimeError(f"{name} has a tangent; this operator has no derivative (use forward_ad.unpack_dual(x).primal)")
 
 
-if torch is not None and hasattr(torch._C, "_cuda_getCurrentRawStream"):
+if torch is not None and hasattr(torch._C, "_cuda_getCurrentRawStream") and hasattr(torch._C, "_cuda_getDevice"):
     _stream_of = torch._C._cuda_getCurrentRawStream  # 1.7 us less a call than the Stream object
+    _current_device = torch._C._cuda_getDevice  # the public one asks first whether there is a GPU
 else:  # pragma: no cover
     def _stream_of(index):
         return torch.cuda.current_stream(index).cuda_stream
+
+    def _current_device():
+        return torch.cuda.current_device()
 
 
 def _launch(t, fn, *args):
     """fn(*args, stream) on the current stream of t's device."""
     index = t.device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         fn(*args, _stream_of(index))
     else:
         with torch.cuda.device(index):
@@ -105,12 +115,13 @@ def _launch(t, fn, *args):
 
 def _optional(t, name):
     """The address of a tensor that may be None: 0 for None only (the kernels refuse a null pointer elsewhere)."""
-    if t is None:
-        return 0
-    p = t.data_ptr()
-    if not p and t.numel():
+    return 0 if t is None else t.data_ptr() or _no_memory(t, name)
+
+
+def _no_memory(t, name):
+    if t.numel():
         raise ValueError(f"{name} has no memory")
-    return p
+    return 0
 
 
 def _new(t):
@@ -233,17 +244,22 @@ def _cache(cache, device=None):
             raise ValueError(f"{name}: an 8-bit cache has scales")
         if not isinstance(s, torch.Tensor) or s.device != dev or s.dtype != torch.float32 or s.shape != k.shape[:3]:
             raise ValueError(f"{name} must be an fp32 tensor of {tuple(k.shape[:3])} on {dev}")
-        _as_stored(s, name)
+        if s.requires_grad or _forward_ad._current_level >= 0 or s.is_neg():
+            _as_stored(s, name)
     return k, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), st + ks.stride() + vs.stride()
 
 
-_rehearsal = threading.local()
+class _Rehearsal(threading.local):
+    why = None
+
+
+_rehearsal = _Rehearsal()
 
 
 @contextlib.contextmanager
 def no_cache_writes(why: str):
     """In this thread :func:`kv_cache_write` raises: for callers that run a module on rows that are no request's."""
-    before, _rehearsal.why = getattr(_rehearsal, "why", None), why
+    before, _rehearsal.why = _rehearsal.why, why
     try:
         yield
     finally:
@@ -268,7 +284,7 @@ def kv_cache_write(cache: KVCache, k, v, slots) -> KVCache:
     the cache is left out (padding).  Slots must not name the same place twice:
     which row's values it would hold is not defined.
     """
-    if getattr(_rehearsal, "why", None):
+    if _rehearsal.why:
         raise RuntimeError(f"the cache is not written: {_rehearsal.why}")
     c, ptrs, cst = _cache(cache)
     dev = c.device

@@ -30,7 +30,7 @@ def test_importing_ops_does_not_load_torch():
 def no_device(monkeypatch):
     """Calls get as far as the native launchers, which refuse before they launch, on a machine without a GPU too."""
     monkeypatch.setattr(ops.token_step, "_stream_of", lambda index: 0)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(ops.token_step, "_current_device", lambda: 0)
 
 
 def fake(*shape, dtype=torch.bfloat16):
