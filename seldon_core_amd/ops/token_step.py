@@ -124,6 +124,23 @@ def _no_memory(t, name):
     return 0
 
 
+def _written(t, name):
+    """Refuse a tensor to write that holds an element twice (an expanded one)."""
+    if 0 in t.stride() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name} holds elements more than once (it is expanded), and is written")
+
+
+def _in_place(out, t):
+    return out is t or out.data_ptr() == t.data_ptr() and out.stride() == t.stride()
+
+
+def _apart(out, t, name, other):
+    """Refuse an output over an input, as far as the host can tell: a common start, or ranges of two contiguous tensors that meet."""
+    a, b = out.data_ptr(), t.data_ptr()
+    if a < b + t.nbytes and b < a + out.nbytes and (a == b or out.is_contiguous() and t.is_contiguous()):
+        raise ValueError(f"{name} lies over {other}")
+
+
 def _new(t):
     """An uninitialised contiguous tensor of t's shape, type and device."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
@@ -180,6 +197,12 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, *, eps: float = 
             _tensor(o, name, 3, (dt,), dev)
             if o.shape != x.shape:
                 raise ValueError(f"{name} must be {tuple(x.shape)}, got {tuple(o.shape)}")
+            _written(o, name)
+            if not _in_place(o, x):
+                _apart(o, x, name, "its input")
+        _apart(oq, k, "out[0]", "k")
+        _apart(ok, q, "out[1]", "q")
+        _apart(oq, ok, "out[0]", "out[1]")
     if T and Hq + Hk:
         _launch(q, _k().qk_norm_rope, q.data_ptr(), k.data_ptr(), oq.data_ptr(), ok.data_ptr(),
                 _optional(q_weight, "q_weight"), _optional(k_weight, "k_weight"), bool(wf32),
@@ -238,7 +261,7 @@ def _cache(cache, device=None):
     if k.dtype in _FLOATS:
         if ks is not None or vs is not None:
             raise ValueError(f"a {k.dtype} cache has no scales")
-        return k, (k.data_ptr(), v.data_ptr(), 0, 0), st + (0,) * 6
+        return k, (k.data_ptr(), v.data_ptr(), 0, 0), st + (1,) * 6
     for s, name in ((ks, "cache.k_scales"), (vs, "cache.v_scales")):
         if s is None:
             raise ValueError(f"{name}: an 8-bit cache has scales")
@@ -297,6 +320,10 @@ def kv_cache_write(cache: KVCache, k, v, slots) -> KVCache:
             raise ValueError(f"{name} must be {(T, heads, dim)}, got {tuple(x.shape)}")
     if dim > 512:
         raise ValueError(f"dim must be at most 512, got {dim}")
+    if 0 in cst:
+        for t, name in zip(cache, ("cache.k", "cache.v", "cache.k_scales", "cache.v_scales")):
+            if t is not None:
+                _written(t, name)
     if T:
         _launch(c, _k().kv_cache_write, (k.data_ptr(), v.data_ptr()), k.stride()[:2] + v.stride()[:2], _TYPE[k.dtype], ptrs,
                 cst, _TYPE[c.dtype], pages, page, slots.data_ptr(), _INDEX[slots.dtype], T, heads, dim)
@@ -387,6 +414,7 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
         _tensor(out, "out", 3, (q.dtype,), dev, contiguous=True)
         if out.shape != q.shape:
             raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+        _apart(out, q, "out", "q")
     lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
     if B:
         n = _attention_workspace(B, H, Hq // H, D, c.dtype.itemsize == 1, W * page, window)
@@ -444,6 +472,10 @@ def lora_add(y, x, A, B, adapters, scales=None, out=None):
         _tensor(out, "out", 2, (dt,), dev)
         if out.shape != y.shape:
             raise ValueError(f"out must be {tuple(y.shape)}, got {tuple(out.shape)}")
+        _written(out, "out")
+        if not _in_place(out, y):
+            _apart(out, y, "out", "y")
+        _apart(out, x, "out", "x")
     if T and M:
         if _lora_workspace is None:
             _lora_workspace = functools.lru_cache(maxsize=1024)(_k().lora_workspace)

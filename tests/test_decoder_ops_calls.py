@@ -427,3 +427,67 @@ def test_lora_add_sorted_rows_in_a_captured_graph():
         torch.cuda.synchronize()
         assert torch.equal(out, eager) and not torch.equal(out, other)
         lora_check(out, y, x, A, B, ids, None)
+
+
+# ------------------------------------------------------------ what is written
+def test_tensors_that_hold_an_element_twice_are_not_written():
+    """An expanded out or cache names the same memory for several rows, which kernels would write in any order."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    f32, i32 = torch.float32, torch.int32
+    with FakeTensorMode():
+        q, k, n, inv = fake(4, 8, 64), fake(4, 2, 64), fake(4, dtype=i32), fake(32, dtype=f32)
+        x, y, A, B, ids = fake(6, 32), fake(6, 48), fake(3, 8, 32), fake(3, 48, 8), fake(6, dtype=i32)
+        pages = fake(1, 16, 2, 64).expand(5, 16, 2, 64)
+        c8 = [fake(5, 16, 2, 64, dtype=torch.int8) for _ in range(2)]
+        for name, call in {
+            r"out\[1\]": lambda: ops.qk_norm_rope(q, k, None, None, n, inv, out=(q, fake(4, 1, 64).expand(4, 2, 64))),
+            "cache.k": lambda: ops.kv_cache_write(ops.KVCache(pages, fake(5, 16, 2, 64)), k, k, n),
+            "cache.v": lambda: ops.kv_cache_write(ops.KVCache(fake(5, 16, 2, 64), pages), k, k, n),
+            "cache.k_scales": lambda: ops.kv_cache_write(ops.KVCache(*c8, fake(5, 16, 1, dtype=f32).expand(5, 16, 2), fake(5, 16, 2, dtype=f32)), k, k, n),
+            "out": lambda: ops.lora_add(y, x, A, B, ids, out=fake(1, 48).expand(6, 48)),
+        }.items():
+            with pytest.raises(ValueError, match=f"^{name} holds elements more than once"):
+                call()
+        # a dimension of one has any stride
+        one = fake(1, 48).as_strided((1, 48), (0, 1))
+        assert ops.token_step._written(one, "out") is None
+
+
+@pytest.mark.gpu
+def test_outputs_over_inputs_are_refused():
+    """The host sees where tensors lie: an output over an input that other workgroups still read is refused, one in its place (where
+    that is allowed) or beside it in one buffer is not."""
+    g, bf = gen(8), torch.bfloat16
+    buf = randn(g, 40, 256, dtype=bf).cuda()
+    y, x, out = buf[:8], buf[8:16], buf[4:12]
+    A, B, ids = randn(g, 2, 8, 256, dtype=bf).cuda(), randn(g, 2, 256, 8, dtype=bf).cuda(), torch.zeros(8, dtype=torch.int32, device="cuda")
+    for o in (x, out):
+        with pytest.raises(ValueError, match="out lies over"):
+            ops.lora_add(y, x, A, B, ids, out=o)
+    with pytest.raises(ValueError, match="out lies over y"):  # the same first element, other rows
+        ops.lora_add(buf.view(20, 512)[:8, :256], buf[30:38], A, B, ids, out=buf[:8])
+    with pytest.raises(ValueError, match="out lies over y"):  # a row further
+        ops.lora_add(y, x, A, B, ids, out=buf[1:9])
+    want = ops.lora_add(y, x, A, B, ids)
+    assert torch.equal(ops.lora_add(y, x, A, B, ids, out=buf[16:24]), want)
+    wide = buf[24:32].reshape(4, 512).repeat(2, 1)
+    a, b = wide[:, :256], wide[:, 256:]
+    want = ops.lora_add(a, b, A, B, ids)
+    assert torch.equal(ops.lora_add(a, b, A, B, ids, out=a), want)  # side by side in one buffer, and in place
+
+    T, D = 4, 64
+    pos, inv = torch.arange(T, device="cuda"), torch.ones(32, device="cuda")
+    q, k = (randn(g, T, 2, D, dtype=bf).cuda() for _ in range(2))
+    for o in ((k, q), (q, q), (k, torch.empty_like(k))):
+        with pytest.raises(ValueError, match="lies over"):
+            ops.qk_norm_rope(q, k, None, None, pos, inv, out=o)
+    both = torch.cat((q, k), 1)
+    want = ops.qk_norm_rope(q, k, None, None, pos, inv)
+    got = ops.qk_norm_rope(both[:, :2], both[:, 2:], None, None, pos, inv, out=(both[:, :2], both[:, 2:]))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    c = ops.kv_cache(4, 4, 2, D)
+    with pytest.raises(ValueError, match="out lies over q"):
+        ops.paged_attention(q, c, torch.zeros((T, 1), dtype=torch.int32, device="cuda"), pos.int(), out=q)
+    e = torch.empty((0, 2, D), dtype=bf, device="cuda")
+    assert ops.qk_norm_rope(e, e, None, None, pos[:0], inv, out=(e, e))[0] is e  # nothing lies over nothing
