@@ -47,6 +47,7 @@ if torch is not None:
     _INDEX = {torch.int32: 0, torch.int64: 1}
     _NEGATED = (torch.float32, torch.float16)  # types that views of complex numbers have
     _Tensor = torch.Tensor
+    _increment_version = torch.autograd.graph.increment_version
 
 _kernels = None
 
@@ -141,6 +142,12 @@ def _apart(out, t, name, other):
         raise ValueError(f"{name} lies over {other}")
 
 
+def _changed(tensors):
+    """Tell autograd, which may have kept them for a backward pass, that tensors of the caller's were written over."""
+    if torch.is_grad_enabled():
+        _increment_version(tensors)
+
+
 def _new(t):
     """An uninitialised contiguous tensor of t's shape, type and device."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
@@ -209,6 +216,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, *, eps: float = 
                 q.stride()[:2] + k.stride()[:2] + oq.stride()[:2] + ok.stride()[:2], T, Hq, Hk, D, _TYPE[dt],
                 positions.data_ptr(), _INDEX[positions.dtype], inv_freq.data_ptr(), inv_freq.dtype == torch.float64,
                 inv_freq.shape[0], interleaved, eps)
+        if out is not None:
+            _changed((oq, ok))
     return oq, ok
 
 
@@ -327,6 +336,7 @@ def kv_cache_write(cache: KVCache, k, v, slots) -> KVCache:
     if T:
         _launch(c, _k().kv_cache_write, (k.data_ptr(), v.data_ptr()), k.stride()[:2] + v.stride()[:2], _TYPE[k.dtype], ptrs,
                 cst, _TYPE[c.dtype], pages, page, slots.data_ptr(), _INDEX[slots.dtype], T, heads, dim)
+        _changed(cache[:2] if c.dtype in _FLOATS else cache)
     return cache
 
 
@@ -408,7 +418,8 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
         raise ValueError(f"page_table holds {W * page} tokens for a request: at least 1, at most 2^30")
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = _new(q)
     else:
         _tensor(out, "out", 3, (q.dtype,), dev, contiguous=True)
@@ -422,6 +433,8 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
         _launch(q, _k().paged_attention, q.data_ptr(), q.stride(0), q.stride(1), _TYPE[q.dtype], ptrs, cst, _TYPE[c.dtype],
                 pages, page, page_table.data_ptr(), page_table.stride(0), W, lengths.data_ptr(), B, H, Hq // H, D, window,
                 D ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), n)
+        if given:
+            _changed((out,))
     return (out, lse) if return_lse else out
 
 
@@ -466,7 +479,8 @@ def lora_add(y, x, A, B, adapters, scales=None, out=None):
         _tensor(scales, "scales", 1, (torch.float32,), dev, contiguous=True)
         if scales.shape[0] != N:
             raise ValueError(f"scales must have {N} values, got {scales.shape[0]}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = _new(y)
     else:
         _tensor(out, "out", 2, (dt,), dev)
@@ -484,6 +498,8 @@ def lora_add(y, x, A, B, adapters, scales=None, out=None):
         _launch(y, _k().lora_add, y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0),
                 A.data_ptr(), B.data_ptr(), adapters.data_ptr(), _INDEX[adapters.dtype],
                 _optional(scales, "scales"), T, K, M, r, N, _TYPE[dt], ws.data_ptr(), n)
+        if given:
+            _changed((out,))
     return out
 
 

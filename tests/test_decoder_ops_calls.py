@@ -491,3 +491,26 @@ def test_outputs_over_inputs_are_refused():
         ops.paged_attention(q, c, torch.zeros((T, 1), dtype=torch.int32, device="cuda"), pos.int(), out=q)
     e = torch.empty((0, 2, D), dtype=bf, device="cuda")
     assert ops.qk_norm_rope(e, e, None, None, pos[:0], inv, out=(e, e))[0] is e  # nothing lies over nothing
+
+
+@pytest.mark.gpu
+def test_writes_are_counted_for_autograd():
+    """What an op of autograd's kept for its backward pass and an operator then writes over raises there, as with torch's own."""
+    g = gen(9)
+    x, A, B = randn(g, 3, 8).cuda(), randn(g, 1, 4, 8).cuda(), randn(g, 1, 8, 4).cuda()
+    ids = torch.zeros(3, dtype=torch.int32, device="cuda")
+    w, buf = torch.ones(8, device="cuda", requires_grad=True), torch.zeros((3, 8), device="cuda")
+    loss = (w * buf).sum()
+    ops.lora_add(buf, x, A, B, ids, out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    q, k, pos, inv = randn(g, 3, 2, 8).cuda(), randn(g, 3, 2, 8).cuda(), ids.clone(), torch.ones(4, device="cuda")
+    before = q._version, k._version
+    ops.qk_norm_rope(q, k, None, None, pos, inv, out=(q, k))
+    assert (q._version, k._version) > before and k._version > before[1]
+    c = ops.kv_cache(2, 4, 2, 8, dtype=torch.int8)
+    before = [t._version for t in c]
+    ops.kv_cache_write(c, q, k, torch.arange(3, device="cuda"))
+    assert all(t._version > b for t, b in zip(c, before))
+    with torch.inference_mode():
+        ops.kv_cache_write(ops.kv_cache(2, 4, 2, 8), q, k, torch.arange(3, device="cuda"))
