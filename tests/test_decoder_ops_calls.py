@@ -514,3 +514,19 @@ def test_writes_are_counted_for_autograd():
     assert all(t._version > b for t, b in zip(c, before))
     with torch.inference_mode():
         ops.kv_cache_write(ops.kv_cache(2, 4, 2, 8), q, k, torch.arange(3, device="cuda"))
+
+
+def test_a_forced_build_compiles_what_is_there_already(monkeypatch):
+    import importlib.util
+    import types
+
+    spec = importlib.util.spec_from_file_location("build_native", os.path.join(ROOT, "tools", "build_native.py"))
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    ran = []
+    monkeypatch.setattr(b, "_needs_build", lambda src, obj: False)
+    monkeypatch.setattr(b, "subprocess", types.SimpleNamespace(run=lambda cmd, **kw: ran.append(cmd) or types.SimpleNamespace(returncode=0, stderr="")))
+    b._compile("kernels/rope.hip", False)
+    assert not ran
+    b._compile("kernels/rope.hip", False, force=True)
+    assert len(ran) == 1 and "+packed" not in " ".join(ran[0]) and "-packed-fp32-ops" in ran[0]

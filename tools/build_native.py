@@ -93,10 +93,10 @@ def _needs_build(src: Path, obj: Path) -> bool:
     return False
 
 
-def _compile(src_rel: str, verbose: bool) -> Path:
+def _compile(src_rel: str, verbose: bool, force: bool = False) -> Path:
     src = CSRC / src_rel
     obj = OBJ / (src_rel.replace("/", "__") + ".o")
-    if not _needs_build(src, obj):
+    if not force and not _needs_build(src, obj):
         return obj
     obj.parent.mkdir(parents=True, exist_ok=True)
     flags = _common_flags() + ["-MMD", "-MF", str(obj.with_suffix(".d"))]
@@ -126,11 +126,12 @@ def _vendor_nghttp2() -> Path:
     return dst
 
 
-def build(jobs: int = 8, verbose: bool = False) -> Path:
+def build(jobs: int = 8, verbose: bool = False, force: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        objs = list(ex.map(lambda s: _compile(s, verbose), LIB_SOURCES))
-        lg_objs = list(ex.map(lambda s: _compile(s, verbose), LOADGEN_SOURCES))
+        objs = list(ex.map(lambda s: _compile(s, verbose, force), LIB_SOURCES))
+        # core/json.cc is the library's too
+        lg_objs = list(ex.map(lambda s: _compile(s, verbose, force and s not in LIB_SOURCES), LOADGEN_SOURCES))
     ng = _vendor_nghttp2()
     out = PKG / ("_C" + _ext_suffix())
     newest = max(o.stat().st_mtime for o in objs)
@@ -159,10 +160,11 @@ def main() -> None:
     ap.add_argument("-j", "--jobs", type=int, default=min(8, os.cpu_count() or 4))
     ap.add_argument("--clean", action="store_true")
     ap.add_argument("--verbose", action="store_true")
+    ap.add_argument("--force", action="store_true", help="compile every source, changed or not")
     a = ap.parse_args()
     if a.clean and BUILD.exists():
         shutil.rmtree(BUILD)
-    out = build(a.jobs, a.verbose)
+    out = build(a.jobs, a.verbose, a.force)
     print(f"built {out.relative_to(ROOT)}")
 
 
