@@ -712,6 +712,7 @@ int splits_of(int64_t rows, int inner, int rank) {
 }  // namespace
 
 int64_t lora_workspace(int64_t rows, int inner, int rank, int adapters) {
+  if (rows < 1) throw std::invalid_argument("lora_add: sizes");
   return int64_t(splits_of(rows, inner, rank)) * rows * 16 * rank_tiles(rank) + (sorts(rows, rank, adapters) ? 4 + 2 * rows : 0);
 }
 

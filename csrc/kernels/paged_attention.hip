@@ -584,6 +584,7 @@ template <class T> void by_cache(const PagedAttentionArgs& a, hipStream_t s) {
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 int grid_of(int batch, int kv_heads, int row_blocks, int dim, bool eight_bit, int64_t max_tokens, int window) {
+  if (batch < 1 || kv_heads < 1 || row_blocks < 1 || max_tokens < 1) throw std::invalid_argument("paged_attention: sizes");
   const int64_t seen = window > 0 && window < max_tokens ? window : max_tokens;
   const int64_t steps = (seen + kStep - 1) / kStep, pairs = int64_t(batch) * kv_heads * row_blocks;
   if (pairs > 0x7fffffff / steps) throw std::invalid_argument("paged_attention: too large for one call");

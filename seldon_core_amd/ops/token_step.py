@@ -414,7 +414,7 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
     W = page_table.shape[1]
     if page_table.shape[0] != B or lengths.shape[0] != B:
         raise ValueError(f"page_table {tuple(page_table.shape)} and lengths {tuple(lengths.shape)} must have {B} rows")
-    if W < 1 or W * page > 1 << 30:
+    if not 1 <= W * page <= 1 << 30:
         raise ValueError(f"page_table holds {W * page} tokens for a request: at least 1, at most 2^30")
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")

@@ -530,3 +530,18 @@ def test_a_forced_build_compiles_what_is_there_already(monkeypatch):
     assert not ran
     b._compile("kernels/rope.hip", False, force=True)
     assert len(ran) == 1 and "+packed" not in " ".join(ran[0]) and "-packed-fp32-ops" in ran[0]
+
+
+def test_sizes_of_nothing_are_refused_not_divided_by(C):
+    """A cache of pages without slots, and workspaces of no tokens or rows: errors, not a division by zero, which ends the process."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    code = ("import torch\nfrom seldon_core_amd import native\nk = native().kernels\n"
+            "for f, a in ((k.paged_attention_workspace, (1, 1, 1, 64, False, 0, 0)), (k.lora_workspace, (0, 64, 8, 1))):\n"
+            "    try:\n        f(*a)\n    except ValueError as e:\n        print(e)\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.count("sizes") == 2, (r.returncode, r.stdout, r.stderr)
+    with FakeTensorMode():
+        c = ops.KVCache(fake(5, 0, 2, 64), fake(5, 0, 2, 64))
+        with pytest.raises(ValueError, match="at least 1"):
+            ops.paged_attention(fake(4, 8, 64), c, fake(4, 3, dtype=torch.int32), fake(4, dtype=torch.int32))
