@@ -418,6 +418,7 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
         raise ValueError(f"page_table holds {W * page} tokens for a request: at least 1, at most 2^30")
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
+    window = min(window, W * page)  # a larger one sees all, and may be no 32-bit number
     given = out is not None
     if not given:
         out = _new(q)

@@ -545,3 +545,27 @@ def test_sizes_of_nothing_are_refused_not_divided_by(C):
         c = ops.KVCache(fake(5, 0, 2, 64), fake(5, 0, 2, 64))
         with pytest.raises(ValueError, match="at least 1"):
             ops.paged_attention(fake(4, 8, 64), c, fake(4, 3, dtype=torch.int32), fake(4, dtype=torch.int32))
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+def test_a_window_larger_than_any_table_sees_all(no_device, monkeypatch):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    seen = []
+    monkeypatch.setattr(ops.token_step, "_attention_workspace", lambda *sizes: seen.append(sizes) or 1)
+    with FakeTensorMode():
+        c, q, table, n = ops.KVCache(fake(5, 16, 2, 64), fake(5, 16, 2, 64)), fake(4, 8, 64), fake(4, 3, dtype=torch.int32), fake(4, dtype=torch.int32)
+        for window in (2 ** 40, 48, 47):
+            with pytest.raises(ValueError):  # by the launcher, as far as a fake call gets
+                ops.paged_attention(q, c, table, n, window=window)
+    assert [s[-1] for s in seen] == [48, 48, 47]
+
+
+@pytest.mark.gpu
+def test_a_window_larger_than_any_table_gives_the_same():
+    g = gen(10)
+    c = ops.kv_cache(20, 16, 2, 64)
+    ops.kv_cache_write(c, *(randn(g, 300, 2, 64, dtype=torch.bfloat16).cuda() for _ in range(2)), torch.arange(300, device="cuda"))
+    q, table = randn(g, 2, 4, 64, dtype=torch.bfloat16).cuda(), torch.arange(20, device="cuda").int().expand(2, 20)
+    n = torch.tensor([300, 77], device="cuda").int()
+    assert torch.equal(ops.paged_attention(q, c, table, n, window=2 ** 40), ops.paged_attention(q, c, table, n))
