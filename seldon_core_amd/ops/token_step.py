@@ -169,7 +169,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, *, eps: float = 
     else is computed in fp32 and rounded once.
 
     Returns the new (q, k), contiguous, or ``out`` = (q, k), which may be the
-    inputs themselves (other overlaps are not allowed).
+    inputs themselves (other overlaps are not allowed).  Sums of squares are
+    fp32: heads with values beyond about 10^18 overflow them and give zeros.
     """
     _tensor(q, "q", 3, _FLOATS)
     dev, dt = q.device, q.dtype
@@ -241,8 +242,14 @@ def kv_cache(pages: int, page_size: int, heads: int, dim: int, dtype=None, devic
     A page keeps the rows of a head together (the tensors are transposed views):
     attention reads one head at a time, and where rows are not whole 128-byte
     lines it would otherwise fetch its neighbours' too (36 requests of 3000
-    tokens, 12 heads: 47 against 68 us at e4m3 and dim 64, 129 against 139 at
-    bf16 and dim 128).
+    tokens, 12 heads, kernels alone: 44 against 67 us at e4m3 and dim 64, 123
+    against 133 at bf16 and dim 128).
+
+    Any dim up to 512 in any of the types can be written and read.
+    :func:`paged_attention` takes bf16, fp16 and 8-bit caches whose dim is at
+    most 256 and a multiple of 8 (of 16 in 8 bits); fp32 caches and other dims
+    are for attention of the caller's own over rows read back.  A dim that is no
+    multiple of 8 is written and read value by value, which is slower.
     """
     dtype = dtype or torch.bfloat16
     if dtype not in _TYPE:
@@ -257,28 +264,30 @@ def kv_cache(pages: int, page_size: int, heads: int, dim: int, dtype=None, devic
 
 
 def _cache(cache, device=None):
-    """Check a cache; -> (k, pointers, strides) as the kernels take them."""
+    """Check a cache; -> (k, its shape, pointers, strides) as the kernels take them."""
     k, v, ks, vs = cache
     _tensor(k, "cache.k", 4, _TYPE, device)
     dev = k.device
     _tensor(v, "cache.v", 4, (k.dtype,), dev)
-    if v.shape != k.shape:
-        raise ValueError(f"cache.k {tuple(k.shape)} and cache.v {tuple(v.shape)} must have one shape")
-    if k.shape[0] * k.shape[1] >= 1 << 31:
+    shape = k.shape
+    if v.shape != shape:
+        raise ValueError(f"cache.k {tuple(shape)} and cache.v {tuple(v.shape)} must have one shape")
+    if shape[0] * shape[1] >= 1 << 31:
         raise ValueError("a cache has at most 2^31 - 1 slots")
     st = k.stride()[:3] + v.stride()[:3]
     if k.dtype in _FLOATS:
         if ks is not None or vs is not None:
             raise ValueError(f"a {k.dtype} cache has no scales")
-        return k, (k.data_ptr(), v.data_ptr(), 0, 0), st + (1,) * 6
+        return k, shape, (k.data_ptr(), v.data_ptr(), 0, 0), st + (1,) * 6
+    rows = shape[:3]
     for s, name in ((ks, "cache.k_scales"), (vs, "cache.v_scales")):
         if s is None:
             raise ValueError(f"{name}: an 8-bit cache has scales")
-        if not isinstance(s, torch.Tensor) or s.device != dev or s.dtype != torch.float32 or s.shape != k.shape[:3]:
-            raise ValueError(f"{name} must be an fp32 tensor of {tuple(k.shape[:3])} on {dev}")
+        if not isinstance(s, _Tensor) or s.shape != rows or s.dtype != torch.float32 or s.device != dev:
+            raise ValueError(f"{name} must be an fp32 tensor of {tuple(rows)} on {dev}")
         if s.requires_grad or _forward_ad._current_level >= 0 or s.is_neg():
             _as_stored(s, name)
-    return k, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), st + ks.stride() + vs.stride()
+    return k, shape, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), st + ks.stride() + vs.stride()
 
 
 class _Rehearsal(threading.local):
@@ -314,19 +323,19 @@ def kv_cache_write(cache: KVCache, k, v, slots) -> KVCache:
     nothing), int8 under the largest value / 127.  A head that holds an infinity
     or a NaN reads back as NaN in 8 bits.  A row whose slot is negative or behind
     the cache is left out (padding).  Slots must not name the same place twice:
-    which row's values it would hold is not defined.
+    it would hold parts of several rows, under the scale of one of them.
     """
     if _rehearsal.why:
         raise RuntimeError(f"the cache is not written: {_rehearsal.why}")
-    c, ptrs, cst = _cache(cache)
+    c, (pages, page, heads, dim), ptrs, cst = _cache(cache)
     dev = c.device
-    pages, page, heads, dim = c.shape
     _tensor(k, "k", 3, _FLOATS, dev)
     _tensor(v, "v", 3, (k.dtype,), dev)
     T = _slots(slots, dev)
+    shape = (T, heads, dim)
     for x, name in ((k, "k"), (v, "v")):
-        if x.shape != (T, heads, dim):
-            raise ValueError(f"{name} must be {(T, heads, dim)}, got {tuple(x.shape)}")
+        if x.shape != shape:
+            raise ValueError(f"{name} must be {shape}, got {tuple(x.shape)}")
     if dim > 512:
         raise ValueError(f"dim must be at most 512, got {dim}")
     if 0 in cst:
@@ -344,8 +353,7 @@ def kv_cache_read(cache: KVCache, slots, dtype=None) -> Tuple:
     """The rows at ``slots`` [T] of a cache as (k, v) [T, heads, dim] in
     ``dtype`` (fp32, fp16 or bf16; the cache's own, or bf16 for an 8-bit one).
     A slot that is negative or behind the cache gives zeros."""
-    c, ptrs, cst = _cache(cache)
-    pages, page, heads, dim = c.shape
+    c, (pages, page, heads, dim), ptrs, cst = _cache(cache)
     dtype = dtype or (c.dtype if c.dtype in _FLOATS else torch.bfloat16)
     if dtype not in _FLOATS:
         raise TypeError(f"dtype must be one of {[str(d) for d in _FLOATS]}, got {dtype}")
@@ -378,7 +386,7 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
     ``q`` [B, Hq, D] (fp16 or bf16, any strides but a contiguous last
     dimension); the ``cache`` is of q's type, float8_e4m3fn or int8, and query
     head h reads its head h // (Hq / H).  ``page_table`` [B, W] int32 (rows may
-    be strided) names each request's pages in order, ``lengths`` [B] int32 how
+    be strided; int32 only, unlike slots) names each request's pages in order, ``lengths`` [B] int32 how
     many tokens it has, its new one among them: that one sees all of them, or
     the last ``window``.  ``scale`` is D ** -0.5 unless given.
 
@@ -400,9 +408,8 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
     """
     _tensor(q, "q", 3, (torch.bfloat16, torch.float16))
     dev = q.device
-    c, ptrs, cst = _cache(cache, dev)
+    c, (pages, page, H, dim), ptrs, cst = _cache(cache, dev)
     B, Hq, D = q.shape
-    pages, page, H, dim = c.shape
     if c.dtype.itemsize != 1 and c.dtype != q.dtype:
         raise TypeError(f"a cache of {c.dtype} does not go with queries of {q.dtype}")
     if dim != D or not H or not Hq or Hq % H:
