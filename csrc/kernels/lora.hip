@@ -22,7 +22,7 @@
 // power of two, which is multiplied back in fp32, so that it cannot overflow.
 //
 // 4096 to 4096 in bf16: 64 rows of 32 adapters of rank 16 take 5.2 + 6.0 us (two chains of waits); 8192 rows of 8
-// adapters of rank 64 take 4.7 (is it sorted?) + 26 + 34 us for 210 MB.
+// adapters of rank 64 take 4.8 (is it sorted?) + 26 to 28 + 34 us for 210 MB; in fp16 4.7 + 26 + 44, in fp32 4.7 + 61 + 93.
 #include <hip/hip_runtime.h>
 
 #include <stdexcept>
@@ -83,9 +83,10 @@ template <class T> __device__ __forceinline__ frag<T> load_masked(const T* base,
 
 // Memory and the matrix instruction want a wave's 16 rows in different lanes.  A load or store serves 16 neighbouring
 // lanes at a time, one cache access for each row among them, so memory has four lanes side by side on a row (lane =
-// 4 row + run); an operand has its rows side by side (lane = 16 run + row).  Loaded in the operand's order the cache's
-// accesses, four times as many, took two thirds of both kernels' time.  So loads are in memory's order, and the lanes
-// are exchanged in registers: to_operand() and, for the fp32 results, to_memory().
+// 4 row + run); an operand has its rows side by side (lane = 16 run + row).  Loaded in the operand's order a wave's load
+// is 64 accesses of the cache, in memory's order 16 (TCP_TOTAL_CACHE_ACCESSES / SQ_INSTS_VMEM_RD), which took lora_down of
+// 8192 rows from 30 to 26 us.  So loads are in memory's order, and the lanes are exchanged in registers: to_operand() and,
+// for the fp32 results, to_memory().
 __device__ __forceinline__ uint32_t from_lane(uint32_t x, int lane) {
   return uint32_t(__builtin_amdgcn_ds_bpermute(lane * 4, int(x)));
 }
@@ -259,7 +260,10 @@ __global__ __launch_bounds__(kSortThreads) void lora_sort(const LoraArgs a) {
 template <class T, int NR, int ROWS> __global__ __launch_bounds__(64 * kDownWaves<ROWS>) void lora_down(const LoraArgs a) {
   extern __shared__ __attribute__((aligned(16))) float part[];  // [kW][ROWS][16 NR + 4]
   constexpr int kW = kDownWaves<ROWS>, NC = (ROWS + 15) / 16, kRow = 16 * NR + 4;
-  constexpr int kAhead = NR == 1 && NC == 1 ? 8 : NR * NC >= 16 ? 2 : 4;  // steps whose loads are under way
+  // Steps whose loads are under way.  With half as many 64 rows of rank 16 / 64 take 4.9 / 7.9 us instead of 5.2 / 8.8, 8192 of
+  // rank 16 / 64 / 128 15.8 / 26.7 / 37.0 instead of 17.0 / 26.2 / 36.2, in fp32 55 instead of 61; with more (12, 4, 8) none
+  // gains and rank 128 runs out of registers (77).
+  constexpr int kAhead = NR == 1 && NC == 1 ? 8 : NR * NC >= 16 ? 2 : 4;
   const int wave = wave_number(), lane = threadIdx.x & 63, n16 = lane & 15, g4 = lane >> 4;
   const int64_t row0 = int64_t(die_order()) * ROWS;  // a die's L2 then holds its rows' adapters once
   Groups groups(a, row0, ROWS, lane);
@@ -737,7 +741,9 @@ void lora_add(LoraArgs a, hipStream_t s) {
     launch_kernel(lora_sort, 1, kSortThreads, size_t(kSortWaves) * (a.adapters + 1) * sizeof(int), s, a);
   }
   // Columns of a workgroup of "up", in tiles of 64: as few as give the chip four workgroups a CU (two of the larger),
-  // since a mixed batch's groups take them one after the other; at most 16.
+  // since a mixed batch's groups take them one after the other; at most 16.  Of the larger ones the registers let a CU hold two
+  // in 16 bits up to rank 32, and in bf16 of even ranks up to 64 (256 registers, none to spare); the others have one at a time,
+  // and the second half of the grid follows the first (8192 rows of rank 64: bf16 34 us, fp16 44).
   const int64_t tiles = (a.outer + 63) / 64;
   const int64_t each = few(a.rows, a.rank) ? ((a.rows + 3) / 4 * tiles + 1023) / 1024 : ((a.rows + 63) / 64 * tiles + 511) / 512;
   a.col_tiles = int(each > 16 ? 16 : each);
