@@ -144,7 +144,7 @@ def _apart(out, t, name, other):
 
 def _changed(tensors):
     """Tell autograd, which may have kept them for a backward pass, that tensors of the caller's were written over."""
-    if torch.is_grad_enabled():
+    if not torch.is_inference_mode_enabled():  # under no_grad too: they may have been kept outside of it
         _increment_version(tensors)
 
 
