@@ -14,8 +14,10 @@ tensors' device, allocates only its outputs and workspace (from torch's
 allocator, so a captured graph keeps its own) and never synchronises: lengths,
 page tables, slots and adapter ids are read on the GPU only.  What the host can
 see (shapes, types, strides, devices, tensors without memory, as tracers use
-them) is checked and refused with ``ValueError`` / ``TypeError``; indices that point outside a cache or a table
-are left out by the kernels as each op says.  The ops are forward only.
+them) is checked and refused with ``ValueError`` / ``TypeError``; indices that
+point outside a cache or a table are left out by the kernels as each op says.
+The ops are forward only (``RuntimeError`` where a gradient or a tangent would
+be lost).
 
 A captured step pads its batch with rows whose slot is -1 (nothing is written)
 and whose length is 0.  :class:`~seldon_core_amd.models.graphed.GraphedModule`
@@ -323,7 +325,8 @@ def kv_cache_write(cache: KVCache, k, v, slots) -> KVCache:
     nothing), int8 under the largest value / 127.  A head that holds an infinity
     or a NaN reads back as NaN in 8 bits.  A row whose slot is negative or behind
     the cache is left out (padding).  Slots must not name the same place twice:
-    it would hold parts of several rows, under the scale of one of them.
+    it would hold parts of several rows, under the scale of one of them; nor may a
+    row be read that is written (``k`` and ``v`` may be other rows of the cache).
     """
     if _rehearsal.why:
         raise RuntimeError(f"the cache is not written: {_rehearsal.why}")
@@ -385,10 +388,10 @@ def paged_attention(q, cache: KVCache, page_table, lengths, *, scale: Optional[f
 
     ``q`` [B, Hq, D] (fp16 or bf16, any strides but a contiguous last
     dimension); the ``cache`` is of q's type, float8_e4m3fn or int8, and query
-    head h reads its head h // (Hq / H).  ``page_table`` [B, W] int32 (rows may
-    be strided; int32 only, unlike slots) names each request's pages in order, ``lengths`` [B] int32 how
-    many tokens it has, its new one among them: that one sees all of them, or
-    the last ``window``.  ``scale`` is D ** -0.5 unless given.
+    head h reads its head h // (Hq / H).  ``page_table`` [B, W] (int32 only; rows
+    may be strided) names each request's pages in order, ``lengths`` [B] (int32
+    only) how many tokens it has, its new one among them: that one sees all of
+    them, or the last ``window``.  ``scale`` is D ** -0.5 unless given.
 
     D is at most 256 and a row of the cache a multiple of 16 bytes (D a multiple
     of 8, of 16 with 8 bits), starting at one.  A length beyond the table counts
@@ -460,7 +463,8 @@ def lora_add(y, x, A, B, adapters, scales=None, out=None):
     [N, M, r], contiguous, r at most 128 (pad a smaller rank with zeros);
     ``adapters`` [T] int32 or int64; ``scales`` [N] fp32.  A row whose adapter is
     negative or behind the last keeps y.  Rows may come in any order; many rows
-    are fastest where those of one adapter lie together.
+    are fastest where those of one adapter lie together (of up to 2000 adapters
+    they are brought together first, of more they are not).
 
     Sums are fp32, with one rounding at the end.  Where a weight of B is infinite
     the result is: with fp32 tensors the infinity (or, next to a 0, the NaN) that

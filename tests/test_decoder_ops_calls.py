@@ -582,3 +582,18 @@ def test_a_window_larger_than_any_table_gives_the_same():
     q, table = randn(g, 2, 4, 64, dtype=torch.bfloat16).cuda(), torch.arange(20, device="cuda").int().expand(2, 20)
     n = torch.tensor([300, 77], device="cuda").int()
     assert torch.equal(ops.paged_attention(q, c, table, n, window=2 ** 40), ops.paged_attention(q, c, table, n))
+
+
+@pytest.mark.gpu
+def test_rows_of_the_cache_itself_move_to_other_slots():
+    """k and v may be views of the cache that is written, where no row is both read and written."""
+    g = gen(11)
+    c = ops.kv_cache(6, 16, 3, 64)
+    rows = [randn(g, 96, 3, 64, dtype=torch.bfloat16).cuda() for _ in range(2)]
+    ops.kv_cache_write(c, *rows, torch.arange(96, device="cuda"))
+    ops.kv_cache_write(c, c.k[1], c.v[1], torch.arange(64, 80, device="cuda"))
+    k, v = ops.kv_cache_read(c, torch.arange(96, device="cuda"))
+    for got, was in ((k, rows[0]), (v, rows[1])):
+        want = was.clone()
+        want[64:80] = was[16:32]
+        assert torch.equal(got, want)
