@@ -145,9 +145,9 @@ def _apart(out, t, name, other):
 
 
 def _changed(tensors):
-    """Tell autograd, which may have kept them for a backward pass, that tensors of the caller's were written over."""
-    if not torch.is_inference_mode_enabled():  # under no_grad too: they may have been kept outside of it
-        _increment_version(tensors)
+    """Tell autograd that tensors of the caller's were written over: a backward pass may have kept them, also where the writing is
+    under no_grad or in inference mode."""
+    _increment_version(tensors)
 
 
 def _new(t):

@@ -521,12 +521,13 @@ def test_writes_without_gradients_are_counted_too():
     """As torch's own in-place operations are: what was kept may be from outside of the no_grad block."""
     g = gen(9)
     x, A, B = randn(g, 3, 8).cuda(), randn(g, 1, 4, 8).cuda(), randn(g, 1, 8, 4).cuda()
-    w, buf = torch.ones(8, device="cuda", requires_grad=True), torch.zeros((3, 8), device="cuda")
-    loss = (w * buf).sum()
-    with torch.no_grad():
-        ops.lora_add(buf, x, A, B, torch.zeros(3, dtype=torch.int32, device="cuda"), out=buf)
-    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
-        loss.backward()
+    for without in (torch.no_grad, torch.inference_mode):
+        w, buf = torch.ones(8, device="cuda", requires_grad=True), torch.zeros((3, 8), device="cuda")
+        loss = (w * buf).sum()
+        with without():
+            ops.lora_add(buf, x, A, B, torch.zeros(3, dtype=torch.int32, device="cuda"), out=buf)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
 
 
 def test_a_forced_build_compiles_what_is_there_already(monkeypatch):
